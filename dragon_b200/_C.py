@@ -117,6 +117,30 @@ SIGNATURES.update({
                                       ctypes.POINTER(AdamWArgs), ctypes.c_void_p, ctypes.c_void_p]),
 })
 
+CODE_NONE, CODE_I8, CODE_E4M3, CODE_E5M2 = range(4)
+SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
+
+
+def _signature(text):
+    """(int, argtypes) of an entry point: p pointer, l int64, i int, f float."""
+    kinds = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float}
+    return ctypes.c_int, [kinds[c] for c in text]
+
+
+SIGNATURES.update({
+    "dgn_rms_norm": _signature("plplpi" "plpil" "ppllf" "iip"),
+    "dgn_rms_norm_grad_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "dgn_rms_norm_grad": _signature("plplplpi" "pppp" "llliip"),
+    "dgn_route": _signature("plpppp" "liiiiiii" "f" "iip"),
+    "dgn_route_grad": _signature("pplpp" "liiii" "f" "iip"),
+    "dgn_expert_plan_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int]),
+    "dgn_expert_plan": _signature("pliippppl" "ip"),
+    "dgn_expert_dispatch": _signature("pllpppp" "liil" "ip"),
+    "dgn_expert_combine": _signature("ppppl" "plill" "iip"),
+    "dgn_expert_combine_grad": _signature("plpppppp" "pliill" "iip"),
+    "dgn_expert_update_bias": _signature("pppifip"),
+})
+
 _lib = None
 
 

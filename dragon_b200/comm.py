@@ -47,6 +47,14 @@ def _stream_ptr(stream, device):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _enter_stream(stream, device):
+    """Context in which `stream` (a torch stream or a raw handle) is current, so
+    that what a call allocates belongs to it."""
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    return torch.cuda.stream(stream)
+
+
 def _check_tensor(t, device):
     if not t.is_cuda or t.device.index != device:
         raise ValueError("tensor must live on cuda:{} (got {})".format(device, t.device))

@@ -1,0 +1,864 @@
+// Operators of a layer of experts: the choice of each token's experts with its
+// backward pass, the counting sort that puts (token, choice) pairs in the order
+// of their experts, the copy of the rows into that order, the weighted sum back
+// with its backward pass, and the update of the balance bias.
+//
+// All are bound by the bytes they move; no matrix product is involved.
+#include <math.h>
+
+#include "dgn_kernels.cuh"
+#include "dgn_ops.h"
+
+namespace {
+
+using namespace dgn;
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChoices = 32;  // one lane of a warp for each
+constexpr int kMaxGroups = 32;
+constexpr float kTiny = 1e-20f;  // keeps the sum that weights are divided by from zero
+constexpr unsigned kFull = 0xffffffffu;
+
+template <typename T> __device__ __forceinline__ float widen(T v) { return static_cast<float>(v); }
+
+// ---- choice ------------------------------------------------------------------------------
+
+struct RouteParams {
+  const char* logits;
+  const float* bias;
+  const uint8_t* mask;
+  int* indices;
+  float* weights;
+  long long tokens, stride;
+  int experts, k, sigmoid, groups, keep, best, renormalize;
+  float scale;
+};
+
+// Keys as whole numbers that sort like the values: 0 is "not to be chosen", NaN comes first.
+__device__ __forceinline__ u64 order_of(double v) {
+  if (isnan(v)) return ~0ull;
+  const u64 bits = (u64)__double_as_longlong(v + 0.0);  // -0 becomes 0
+  return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+
+// Largest key of a warp and the lowest index that has it.
+__device__ __forceinline__ void first_largest(u64* key, int* index) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const u64 k = __shfl_xor_sync(kFull, *key, d);
+    const int i = __shfl_xor_sync(kFull, *index, d);
+    if (k > *key || (k == *key && i < *index)) {
+      *key = k;
+      *index = i;
+    }
+  }
+}
+
+// One warp for a token, N experts for a lane: lane l holds experts l, l + 32, ...
+template <typename T, int N>
+__global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long token = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  int* indices = p.indices + token * p.k;
+  float* weights = p.weights + token * p.k;
+  if (p.mask && !p.mask[token]) {
+    if (lane < p.k) {
+      indices[lane] = -1;
+      weights[lane] = 0.f;
+    }
+    return;
+  }
+  const T* row = reinterpret_cast<const T*>(p.logits) + token * p.stride;
+  double score[N];
+  u64 key[N];
+  double top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    score[i] = e < p.experts ? (double)widen(row[e]) : -INFINITY;
+    key[i] = isinf(score[i]) && score[i] < 0 ? 0 : order_of(score[i]);
+    top = fmax(top, score[i]);
+  }
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) score[i] = 1.0 / (1.0 + exp(-score[i]));
+  } else {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      score[i] = key[i] ? exp(score[i] - top) : 0.0;
+      sum += score[i];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+#pragma unroll
+    for (int i = 0; i < N; ++i) score[i] = key[i] ? score[i] / sum : 0.0;
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = i * 32 + lane;
+      if (!key[i]) continue;
+      const double v = score[i] + (double)p.bias[e];
+      key[i] = isinf(v) && v < 0 ? 0 : order_of(v);
+    }
+  }
+  if (p.groups > 1) {
+    const int width = p.experts / p.groups;
+    const bool by_key = p.bias || p.best == 1;  // otherwise the score is what is added up
+    u64 mine = 0;  // lane g: the value of group g
+    for (int g = 0; g < p.groups; ++g) {
+      u64 a = 0, b = 0;  // the two largest, by order
+      int ia = kMaxExperts, ib = kMaxExperts;
+      double va = 0.0, vb = 0.0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = i * 32 + lane;
+        if (e / width != g || !key[i]) continue;
+        const double v = p.bias ? score[i] + (double)p.bias[e] : score[i];
+        const u64 o = by_key ? key[i] : order_of(v);
+        if (o > a) {
+          b = a; ib = ia; vb = va;
+          a = o; ia = e; va = v;
+        } else if (o > b) {
+          b = o; ib = e; vb = v;
+        }
+      }
+      u64 k1 = a;
+      int i1 = ia;
+      first_largest(&k1, &i1);
+      if (p.best == 1 || !k1) {
+        if (lane == g) mine = k1;
+        continue;
+      }
+      const int owner1 = __ffs(__ballot_sync(kFull, a == k1 && ia == i1)) - 1;
+      const double v1 = __shfl_sync(kFull, va, owner1);
+      if (lane == owner1) { a = b; ia = ib; va = vb; }
+      u64 k2 = a;
+      int i2 = ia;
+      first_largest(&k2, &i2);
+      const int owner2 = __ffs(__ballot_sync(kFull, a == k2 && ia == i2)) - 1;
+      const double v2 = __shfl_sync(kFull, va, owner2);
+      if (lane == g) mine = order_of(k2 ? v1 + v2 : v1);
+    }
+    unsigned kept = 0;
+    for (int n = 0; n < p.keep; ++n) {
+      u64 k1 = mine;
+      int g = lane;
+      first_largest(&k1, &g);
+      if (!k1) break;
+      kept |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!(kept >> min((i * 32 + lane) / width, 31) & 1)) key[i] = 0;
+  }
+  int index = -1;
+  float s = 0.f;
+  for (int n = 0; n < p.k; ++n) {
+    u64 best = 0;
+    int at = kMaxExperts;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i * 32 + lane;
+        v = (float)score[i];
+      }
+    int e = at;
+    first_largest(&best, &e);
+    if (!best) break;
+    const float chosen = __shfl_sync(kFull, v, e & 31);
+    if (lane == n) {
+      index = e;
+      s = chosen;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane == e) key[i] = 0;
+  }
+  float w = s;
+  if (p.renormalize) {
+    float sum = s;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+    w = s / (sum + kTiny);
+  }
+  if (lane < p.k) {
+    indices[lane] = index;
+    weights[lane] = index < 0 ? 0.f : w * p.scale;
+  }
+}
+
+struct RouteGradParams {
+  const float* grad_weights;
+  const char* logits;
+  const int* indices;
+  char* grad;
+  long long tokens, stride;
+  int experts, k, sigmoid, renormalize;
+  float scale;
+};
+
+template <typename T, int N>
+__global__ void __launch_bounds__(128) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long token = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  const T* row = reinterpret_cast<const T*>(p.logits) + token * p.stride;
+  T* grad = reinterpret_cast<T*>(p.grad) + token * p.experts;
+  float score[N];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    score[i] = e < p.experts ? widen(row[e]) : -INFINITY;
+    top = fmaxf(top, score[i]);
+  }
+  // The chosen experts: lane j < k holds choice j.
+  int index = lane < p.k ? p.indices[token * p.k + lane] : -1;
+  if (index >= p.experts) index = -1;
+  float ds = index < 0 ? 0.f : p.scale * p.grad_weights[token * p.k + lane];
+  if (index < 0) index = -1;
+  if (!__ballot_sync(kFull, index >= 0)) {  // a padded token: whatever its logits hold, no gradient
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane < p.experts) grad[i * 32 + lane] = T(0.f);
+    return;
+  }
+  const float logit = index < 0 ? -INFINITY : widen(row[index]);
+  float mine;
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {  // s (1 - s) without the cancellation near 1
+      const float t = expf(-fabsf(score[i]));
+      score[i] = t / ((1.f + t) * (1.f + t));
+    }
+    mine = index < 0 ? 0.f : 1.f / (1.f + expf(-logit));
+  } else {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      score[i] = score[i] == -INFINITY ? 0.f : expf(score[i] - top);
+      sum += score[i];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+#pragma unroll
+    for (int i = 0; i < N; ++i) score[i] = score[i] == 0.f ? 0.f : score[i] / sum;
+    mine = index < 0 || logit == -INFINITY ? 0.f : expf(logit - top) / sum;
+  }
+  if (p.renormalize) {
+    float total = mine, dot = ds * mine;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      total += __shfl_xor_sync(kFull, total, d);
+      dot += __shfl_xor_sync(kFull, dot, d);
+    }
+    total += kTiny;
+    ds = index < 0 ? 0.f : (ds - dot / total) / total;
+  }
+  float dot = ds * mine;
+  if (p.sigmoid) {
+    dot = 0.f;
+  } else {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
+  }
+  float direct[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) direct[i] = 0.f;
+  for (int j = 0; j < p.k; ++j) {
+    const int e = __shfl_sync(kFull, index, j);
+    const float d = __shfl_sync(kFull, ds, j);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * 32 + lane == e) direct[i] += d;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    const float s = score[i];
+    if (e < p.experts) grad[e] = T(p.sigmoid ? direct[i] * s : s * (direct[i] - dot));
+  }
+}
+
+// ---- plan ----------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanBlocks = 148;
+constexpr int kSlotsOfBlock = 4096;  // slots that one block counts before another joins
+
+int plan_blocks(int64_t slots) {
+  const int64_t n = ceil_div(slots, kSlotsOfBlock);
+  return (int)(n < 1 ? 1 : n < kPlanBlocks ? n : kPlanBlocks);
+}
+
+struct PlanParams {
+  const int* indices;
+  int* counts;
+  int* offsets;
+  int* positions;
+  int* parts;  // [gridDim.x][experts]: how often each block's slots ask for each expert
+  long long slots, span;  // span: slots of a block, a multiple of 32
+  int experts, align;
+};
+
+__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int hist[];
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  const long long first = blockIdx.x * p.span, last = min(first + p.span, p.slots);
+  for (long long s = first + threadIdx.x; s < last; s += blockDim.x) {
+    const int e = p.indices[s];
+    if (e >= 0 && e < p.experts) atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.parts[(long long)blockIdx.x * p.experts + e] = hist[e];
+}
+
+// Every block adds up the counts of the blocks before it, then ranks its own slots: warp w takes the w-th run of them.
+__global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ int hist[];  // [kPlanWarps][experts], then the place of each warp's next slot of an expert
+  __shared__ int carry[kPlanWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, experts = p.experts;
+  for (int i = threadIdx.x; i < kPlanWarps * experts; i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  const long long first = blockIdx.x * p.span, last = min(first + p.span, p.slots);
+  const long long run = (p.span / 32 + kPlanWarps - 1) / kPlanWarps * 32;
+  const long long begin = min(first + warp * run, last), end = min(begin + run, last);
+  for (long long s = begin + lane; s < end; s += 32) {
+    const int e = p.indices[s];
+    if (e >= 0 && e < experts) atomicAdd(&hist[warp * experts + e], 1);
+  }
+  __syncthreads();
+  // Block starts: a scan of the aligned totals over the experts, two experts for a thread.
+  int total[2] = {0, 0}, before[2] = {0, 0}, blocks[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = threadIdx.x * 2 + i;
+    if (e < experts) {
+      if (gridDim.x == 1) {
+        for (int w = 0; w < kPlanWarps; ++w) total[i] += hist[w * experts + e];
+      } else {
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+          const int n = p.parts[(long long)b * experts + e];
+          if (b < (int)blockIdx.x) before[i] += n;
+          total[i] += n;
+        }
+      }
+    }
+    blocks[i] = (total[i] + p.align - 1) / p.align * p.align;
+  }
+  int sum = blocks[0] + blocks[1], scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(kFull, scan, d);
+    if (lane >= d) scan += v;
+  }
+  if (lane == 31) carry[warp] = scan;
+  __syncthreads();
+  int start = scan - sum;
+  for (int w = 0; w < warp; ++w) start += carry[w];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = threadIdx.x * 2 + i;
+    if (e < experts) {
+      if (blockIdx.x == 0) {
+        p.counts[e] = total[i];
+        p.offsets[e] = start;
+        if (e == experts - 1) p.offsets[experts] = start + blocks[i];
+      }
+      int next = start + before[i];
+      for (int w = 0; w < kPlanWarps; ++w) {
+        const int n = hist[w * experts + e];
+        hist[w * experts + e] = next;
+        next += n;
+      }
+      start += blocks[i];
+    }
+  }
+  __syncthreads();
+  int* next = hist + warp * experts;
+  for (long long s = begin; s < end; s += 32) {
+    const int e = s + lane < end ? p.indices[s + lane] : -1;
+    const bool there = e >= 0 && e < experts;
+    const unsigned same = __match_any_sync(kFull, there ? e : -1);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    const int base = there ? next[e] : 0;
+    __syncwarp();
+    if (there && rank == 0) next[e] = base + __popc(same);
+    __syncwarp();
+    if (s + lane < end) p.positions[s + lane] = there ? base + rank : -1;
+  }
+}
+
+// ---- moves -----------------------------------------------------------------------------------
+
+struct MoveParams {
+  const char* x;
+  const int* positions;
+  const int* counts;
+  const int* offsets;
+  char* out;
+  long long tokens, x_stride, row_bytes, capacity;  // bytes
+  int k, experts;
+};
+
+// Zeros in the rows of an expert's block that no slot uses.
+template <typename U>
+__device__ void clear_rows(char* out, const int* counts, const int* offsets, int e, long long row_bytes,
+                           long long capacity) {
+  const long long first = max(0ll, (long long)offsets[e] + counts[e]), last = min((long long)offsets[e + 1], capacity);
+  const long long n = row_bytes / (long long)sizeof(U);
+  for (long long r = first; r < last; ++r)
+    for (long long i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<U*>(out + r * row_bytes)[i] = U{};
+}
+
+// A block for a token, then one for each expert's unused rows.
+template <typename U>
+__global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ MoveParams p) {
+  if (blockIdx.x >= p.tokens) {
+    clear_rows<U>(p.out, p.counts, p.offsets, (int)(blockIdx.x - p.tokens), p.row_bytes, p.capacity);
+    return;
+  }
+  const long long t = blockIdx.x;
+  const U* from = reinterpret_cast<const U*>(p.x + t * p.x_stride);
+  const long long n = p.row_bytes / (long long)sizeof(U);
+  for (long long i = threadIdx.x; i < n; i += blockDim.x) {
+    const U v = from[i];
+    for (int j = 0; j < p.k; ++j) {
+      const long long at = p.positions[t * p.k + j];
+      if (at >= 0 && at < p.capacity) reinterpret_cast<U*>(p.out + at * p.row_bytes)[i] = v;
+    }
+  }
+}
+
+struct CombineParams {
+  const char* rows;
+  const int* positions;
+  const float* weights;
+  const char* residual;
+  char* out;
+  long long tokens, cols, capacity, residual_stride;
+  int k;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 part(const char* row, long long c, long long cols) {
+  if (VEC) return *reinterpret_cast<const uint4*>(row + c * (long long)sizeof(T));
+  uint4 v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::E; ++i)
+    if (c + i < cols) reinterpret_cast<T*>(&v)[i] = reinterpret_cast<const T*>(row)[c + i];
+  return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void put(char* row, long long c, long long cols, uint4 v) {
+  if (VEC) {
+    *reinterpret_cast<uint4*>(row + c * (long long)sizeof(T)) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < Elem<T>::E; ++i)
+    if (c + i < cols) reinterpret_cast<T*>(row)[c + i] = reinterpret_cast<const T*>(&v)[i];
+}
+
+// A block for a token.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
+  constexpr int E = Elem<T>::E;
+  const long long t = blockIdx.x, row_bytes = p.cols * (long long)sizeof(T);
+  for (long long c = threadIdx.x * E; c < p.cols; c += blockDim.x * E) {
+    float sum[E], a[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+      const long long at = p.positions[t * p.k + j];
+      if (at < 0 || at >= p.capacity) continue;
+      const float w = p.weights ? p.weights[t * p.k + j] : 1.f;
+      Elem<T>::unpack(part<T, VEC>(p.rows + at * row_bytes, c, p.cols), a);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] = fmaf(w, a[e], sum[e]);
+    }
+    if (p.residual) {
+      Elem<T>::unpack(part<T, VEC>(p.residual + t * p.residual_stride * (long long)sizeof(T), c, p.cols), a);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] += a[e];
+    }
+    put<T, VEC>(p.out + t * row_bytes, c, p.cols, Elem<T>::pack(sum));
+  }
+}
+
+struct CombineGradParams {
+  const char* grad_out;
+  const char* rows;
+  const int* positions;
+  const float* weights;
+  const int* counts;
+  const int* offsets;
+  char* grad_rows;
+  float* grad_weights;
+  long long tokens, cols, capacity, grad_out_stride;
+  int k, experts;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) combine_grad_kernel(const __grid_constant__ CombineGradParams p) {
+  constexpr int E = Elem<T>::E;
+  __shared__ float slot[8];
+  const long long row_bytes = p.cols * (long long)sizeof(T);
+  if (blockIdx.x >= p.tokens) {
+    const int e = (int)(blockIdx.x - p.tokens);
+    if (VEC) clear_rows<uint4>(p.grad_rows, p.counts, p.offsets, e, row_bytes, p.capacity);
+    else clear_rows<T>(p.grad_rows, p.counts, p.offsets, e, row_bytes, p.capacity);
+    return;
+  }
+  const long long t = blockIdx.x;
+  const char* grad = p.grad_out + t * p.grad_out_stride * (long long)sizeof(T);
+  for (int j = 0; j < p.k; ++j) {
+    const long long at = p.positions[t * p.k + j];
+    float dot = 0.f;
+    if (at >= 0 && at < p.capacity) {
+      const float w = p.weights[t * p.k + j];
+      for (long long c = threadIdx.x * E; c < p.cols; c += blockDim.x * E) {
+        float a[E], b[E];
+        Elem<T>::unpack(part<T, VEC>(grad, c, p.cols), a);
+        Elem<T>::unpack(part<T, VEC>(p.rows + at * row_bytes, c, p.cols), b);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          dot = fmaf(a[e], b[e], dot);
+          a[e] *= w;
+        }
+        put<T, VEC>(p.grad_rows + at * row_bytes, c, p.cols, Elem<T>::pack(a));
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < (int)blockDim.x >> 5; ++w) dot += slot[w];
+      p.grad_weights[t * p.k + j] = dot;
+    }
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(1024) update_bias_kernel(const float* bias, const int* counts, float* out, int experts,
+                                                           float rate) {
+  __shared__ long long slot[32];
+  const int e = threadIdx.x, lane = e & 31;
+  const long long mine = e < experts ? counts[e] : 0;
+  long long total = mine;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
+  if (lane == 0) slot[e >> 5] = total;
+  __syncthreads();
+  total = slot[lane];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
+  if (e >= experts) return;
+  const long long lack = total - (long long)experts * mine;
+  out[e] = bias[e] + (lack > 0 ? rate : lack < 0 ? -rate : 0.f);
+}
+
+// ---- kernel choice -----------------------------------------------------------------------------
+
+template <typename T>
+const void* route_fn(int experts) {
+  if (experts <= 64) return (const void*)route_kernel<T, 2>;
+  if (experts <= 128) return (const void*)route_kernel<T, 4>;
+  if (experts <= 256) return (const void*)route_kernel<T, 8>;
+  if (experts <= 512) return (const void*)route_kernel<T, 16>;
+  return (const void*)route_kernel<T, 32>;
+}
+template <typename T>
+const void* route_grad_fn(int experts) {
+  if (experts <= 64) return (const void*)route_grad_kernel<T, 2>;
+  if (experts <= 128) return (const void*)route_grad_kernel<T, 4>;
+  if (experts <= 256) return (const void*)route_grad_kernel<T, 8>;
+  if (experts <= 512) return (const void*)route_grad_kernel<T, 16>;
+  return (const void*)route_grad_kernel<T, 32>;
+}
+template <typename T>
+const void* combine_fn(bool vec) {
+  return vec ? (const void*)combine_kernel<T, true> : (const void*)combine_kernel<T, false>;
+}
+template <typename T>
+const void* combine_grad_fn(bool vec) {
+  return vec ? (const void*)combine_grad_kernel<T, true> : (const void*)combine_grad_kernel<T, false>;
+}
+
+int check_route(int64_t tokens, int64_t stride, int experts, int k, int score, int dtype) {
+  if (!float_dtype(dtype)) return report_error(DGN_ERR_UNSUPPORTED, "logits are float16, bfloat16 or float32");
+  if (tokens < 0 || tokens > INT32_MAX) return report_error(DGN_ERR_ARG, "a call takes 0..2^31-1 tokens");
+  if (experts < 1 || experts > kMaxExperts) return report_error(DGN_ERR_ARG, "a call takes 1..1024 experts");
+  if (k < 1 || k > kMaxChoices || k > experts)
+    return report_error(DGN_ERR_ARG, "k must be 1..32 and at most the number of experts");
+  if (score != DGN_SCORE_SOFTMAX && score != DGN_SCORE_SIGMOID) return report_error(DGN_ERR_ARG, "unknown score");
+  if (stride < experts) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
+  return DGN_OK;
+}
+
+int check_move(int64_t tokens, int k, int64_t capacity, int64_t row) {
+  if (tokens < 0 || k < 1 || k > kMaxChoices || tokens * k > INT32_MAX)
+    return report_error(DGN_ERR_ARG, "a token has 1..32 choices, a call fewer than 2^31");
+  if (capacity < 0 || capacity > INT32_MAX) return report_error(DGN_ERR_ARG, "capacity must be 0..2^31-1 rows");
+  if (row < 1 || row > INT32_MAX) return report_error(DGN_ERR_ARG, "rows must not be empty or pass 2^31-1");
+  return DGN_OK;
+}
+
+int check_experts(int experts) {
+  if (experts < 1 || experts > kMaxExperts) return report_error(DGN_ERR_ARG, "a call takes 1..1024 experts");
+  return DGN_OK;
+}
+
+int null_pointer(const char* message) { return report_error(DGN_ERR_ARG, message); }
+int misaligned() { return report_error(DGN_ERR_ARG, "a pointer is not aligned to its element size"); }
+
+}  // namespace
+
+#define DGN_ON(device) \
+  OnDevice on(device); \
+  if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()))
+
+extern "C" int dgn_route(const void* logits, int64_t stride, const float* bias, const uint8_t* mask, int32_t* indices,
+                         float* weights, int64_t tokens, int experts, int k, int score, int groups, int keep, int best,
+                         int renormalize, float scale, int dtype, int device, void* stream) {
+  int rc = check_route(tokens, stride, experts, k, score, dtype);
+  if (rc != DGN_OK) return rc;
+  if (groups < 1 || groups > kMaxGroups || experts % groups != 0)
+    return report_error(DGN_ERR_ARG, "groups must be 1..32 and divide the number of experts");
+  if (keep < 1 || keep > groups) return report_error(DGN_ERR_ARG, "at least one group is kept and at most all");
+  if (best != 1 && best != 2) return report_error(DGN_ERR_ARG, "a group is valued by its best 1 or 2 experts");
+  if (tokens == 0) return DGN_OK;
+  if (!logits || !indices || !weights) return null_pointer("dgn_route: null pointer");
+  if (!aligned(logits, dgn_dtype_size(dtype)) || !aligned(bias, 4) || !aligned(indices, 4) || !aligned(weights, 4))
+    return misaligned();
+  RouteParams p;
+  p.logits = static_cast<const char*>(logits);
+  p.bias = bias;
+  p.mask = mask;
+  p.indices = indices;
+  p.weights = weights;
+  p.tokens = tokens;
+  p.stride = stride;
+  p.experts = experts;
+  p.k = k;
+  p.sigmoid = score == DGN_SCORE_SIGMOID;
+  p.groups = groups;
+  p.keep = keep;
+  p.best = best;
+  p.renormalize = renormalize != 0;
+  p.scale = scale;
+  const void* fn = dtype == DGN_F32   ? route_fn<float>(experts)
+                   : dtype == DGN_F16 ? route_fn<__half>(experts)
+                                      : route_fn<__nv_bfloat16>(experts);
+  DGN_ON(device);
+  void* args[] = {&p};
+  return launch(fn, dim3((unsigned)ceil_div(tokens, 4)), dim3(128), 0, stream, args);
+}
+
+extern "C" int dgn_route_grad(const float* grad_weights, const void* logits, int64_t stride, const int32_t* indices,
+                              void* grad_logits, int64_t tokens, int experts, int k, int score, int renormalize,
+                              float scale, int dtype, int device, void* stream) {
+  int rc = check_route(tokens, stride, experts, k, score, dtype);
+  if (rc != DGN_OK) return rc;
+  if (tokens == 0) return DGN_OK;
+  if (!grad_weights || !logits || !indices || !grad_logits) return null_pointer("dgn_route_grad: null pointer");
+  const size_t es = dgn_dtype_size(dtype);
+  if (!aligned(logits, es) || !aligned(grad_logits, es) || !aligned(indices, 4) || !aligned(grad_weights, 4))
+    return misaligned();
+  RouteGradParams p;
+  p.grad_weights = grad_weights;
+  p.logits = static_cast<const char*>(logits);
+  p.indices = indices;
+  p.grad = static_cast<char*>(grad_logits);
+  p.tokens = tokens;
+  p.stride = stride;
+  p.experts = experts;
+  p.k = k;
+  p.sigmoid = score == DGN_SCORE_SIGMOID;
+  p.renormalize = renormalize != 0;
+  p.scale = scale;
+  const void* fn = dtype == DGN_F32   ? route_grad_fn<float>(experts)
+                   : dtype == DGN_F16 ? route_grad_fn<__half>(experts)
+                                      : route_grad_fn<__nv_bfloat16>(experts);
+  DGN_ON(device);
+  void* args[] = {&p};
+  return launch(fn, dim3((unsigned)ceil_div(tokens, 4)), dim3(128), 0, stream, args);
+}
+
+extern "C" int64_t dgn_expert_plan_workspace(int64_t slots, int experts) {
+  const int blocks = plan_blocks(slots);
+  return blocks == 1 || experts < 1 ? 0 : (int64_t)blocks * experts * (int64_t)sizeof(int);
+}
+
+extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int experts, int align, int32_t* counts,
+                               int32_t* offsets, int32_t* positions, void* workspace, int64_t workspace_bytes,
+                               int device, void* stream) {
+  int rc = check_experts(experts);
+  if (rc != DGN_OK) return rc;
+  if (slots < 0 || slots > INT32_MAX) return report_error(DGN_ERR_ARG, "a call takes 0..2^31-1 slots");
+  if (align < 1 || slots + (slots < experts ? slots : experts) * ((int64_t)align - 1) > INT32_MAX)
+    return report_error(DGN_ERR_ARG, "align must be positive and the rows fewer than 2^31");
+  if (!counts || !offsets || (slots && (!indices || !positions))) return null_pointer("dgn_expert_plan: null pointer");
+  if (!aligned(indices, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(positions, 4) ||
+      !aligned(workspace, 4))
+    return misaligned();
+  const int64_t need = dgn_expert_plan_workspace(slots, experts);
+  if (need && (!workspace || workspace_bytes < need))
+    return report_error(DGN_ERR_ARG, "dgn_expert_plan: workspace too small");
+  PlanParams p;
+  p.indices = indices;
+  p.counts = counts;
+  p.offsets = offsets;
+  p.positions = positions;
+  p.parts = static_cast<int*>(workspace);
+  p.slots = slots;
+  p.experts = experts;
+  p.align = align;
+  const int blocks = plan_blocks(slots);
+  p.span = ceil_div(ceil_div(slots, blocks), 32) * 32;
+  DGN_ON(device);
+  void* args[] = {&p};
+  if (blocks > 1) {
+    rc = launch((const void*)plan_count_kernel, dim3(blocks), dim3(kPlanThreads), experts * sizeof(int), stream, args);
+    if (rc != DGN_OK) return rc;
+  }
+  const int smem = kPlanWarps * experts * (int)sizeof(int);
+  if (smem > 48 << 10) {
+    cudaError_t e = cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
+  }
+  return launch((const void*)plan_place_kernel, dim3(blocks), dim3(kPlanThreads), smem, stream, args);
+}
+
+extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_bytes, const int32_t* positions,
+                                   const int32_t* counts, const int32_t* offsets, void* out, int64_t tokens, int k,
+                                   int experts, int64_t capacity, int device, void* stream) {
+  int rc = check_move(tokens, k, capacity, row_bytes);
+  if (rc == DGN_OK) rc = check_experts(experts);
+  if (rc != DGN_OK) return rc;
+  if (x_stride < row_bytes) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
+  if (tokens == 0 || capacity == 0) return DGN_OK;
+  if (!x || !positions || !counts || !offsets || !out) return null_pointer("dgn_expert_dispatch: null pointer");
+  if (!aligned(positions, 4) || !aligned(counts, 4) || !aligned(offsets, 4)) return misaligned();
+  MoveParams p;
+  p.x = static_cast<const char*>(x);
+  p.positions = positions;
+  p.counts = counts;
+  p.offsets = offsets;
+  p.out = static_cast<char*>(out);
+  p.tokens = tokens;
+  p.x_stride = x_stride;
+  p.row_bytes = row_bytes;
+  p.capacity = capacity;
+  p.k = k;
+  p.experts = experts;
+  // The widest word that divides the addresses, the strides and the row.
+  const auto fits = [&](int w) { return aligned(x, w) && aligned(out, w) && x_stride % w == 0 && row_bytes % w == 0; };
+  const void* fn = fits(16)  ? (const void*)dispatch_kernel<uint4>
+                   : fits(8) ? (const void*)dispatch_kernel<uint2>
+                   : fits(4) ? (const void*)dispatch_kernel<unsigned>
+                   : fits(2) ? (const void*)dispatch_kernel<unsigned short>
+                             : (const void*)dispatch_kernel<unsigned char>;
+  DGN_ON(device);
+  void* args[] = {&p};
+  return launch(fn, dim3((unsigned)(tokens + experts)), dim3(256), 0, stream, args);
+}
+
+extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, const float* weights,
+                                  const void* residual, int64_t residual_stride, void* out, int64_t tokens, int k,
+                                  int64_t cols, int64_t capacity, int dtype, int device, void* stream) {
+  int rc = check_move(tokens, k, capacity, cols);
+  if (rc != DGN_OK) return rc;
+  if (!float_dtype(dtype)) return report_error(DGN_ERR_UNSUPPORTED, "rows are float16, bfloat16 or float32");
+  if (residual && residual_stride < cols) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
+  if (tokens == 0) return DGN_OK;
+  if ((!rows && capacity) || !positions || !out) return null_pointer("dgn_expert_combine: null pointer");
+  const int es = (int)dgn_dtype_size(dtype), elems = 16 / es;
+  if (!aligned(rows, es) || !aligned(residual, es) || !aligned(out, es) || !aligned(positions, 4) || !aligned(weights, 4))
+    return misaligned();
+  const bool vec = cols % elems == 0 && aligned(rows, 16) && aligned(out, 16) &&
+                   (!residual || (aligned(residual, 16) && residual_stride % elems == 0));
+  CombineParams p;
+  p.rows = static_cast<const char*>(rows);
+  p.positions = positions;
+  p.weights = weights;
+  p.residual = static_cast<const char*>(residual);
+  p.out = static_cast<char*>(out);
+  p.tokens = tokens;
+  p.cols = cols;
+  p.capacity = capacity;
+  p.residual_stride = residual_stride;
+  p.k = k;
+  const void* fn = dtype == DGN_F32   ? combine_fn<float>(vec)
+                   : dtype == DGN_F16 ? combine_fn<__half>(vec)
+                                      : combine_fn<__nv_bfloat16>(vec);
+  DGN_ON(device);
+  void* args[] = {&p};
+  return launch(fn, dim3((unsigned)tokens), dim3(256), 0, stream, args);
+}
+
+extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_stride, const void* rows,
+                                       const int32_t* positions, const float* weights, const int32_t* counts,
+                                       const int32_t* offsets, void* grad_rows, float* grad_weights, int64_t tokens,
+                                       int k, int experts, int64_t cols, int64_t capacity, int dtype, int device,
+                                       void* stream) {
+  int rc = check_move(tokens, k, capacity, cols);
+  if (rc == DGN_OK) rc = check_experts(experts);
+  if (rc != DGN_OK) return rc;
+  if (!float_dtype(dtype)) return report_error(DGN_ERR_UNSUPPORTED, "rows are float16, bfloat16 or float32");
+  if (grad_out_stride < cols) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
+  if (tokens == 0) return DGN_OK;
+  if (!grad_out || !positions || !weights || !counts || !offsets || !grad_weights || (capacity && (!rows || !grad_rows)))
+    return null_pointer("dgn_expert_combine_grad: null pointer");
+  const int es = (int)dgn_dtype_size(dtype), elems = 16 / es;
+  if (!aligned(grad_out, es) || !aligned(rows, es) || !aligned(grad_rows, es) || !aligned(positions, 4) ||
+      !aligned(weights, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(grad_weights, 4))
+    return misaligned();
+  const bool vec = cols % elems == 0 && aligned(grad_out, 16) && grad_out_stride % elems == 0 && aligned(rows, 16) &&
+                   aligned(grad_rows, 16);
+  CombineGradParams p;
+  p.grad_out = static_cast<const char*>(grad_out);
+  p.rows = static_cast<const char*>(rows);
+  p.positions = positions;
+  p.weights = weights;
+  p.counts = counts;
+  p.offsets = offsets;
+  p.grad_rows = static_cast<char*>(grad_rows);
+  p.grad_weights = grad_weights;
+  p.tokens = tokens;
+  p.cols = cols;
+  p.capacity = capacity;
+  p.grad_out_stride = grad_out_stride;
+  p.k = k;
+  p.experts = experts;
+  const void* fn = dtype == DGN_F32   ? combine_grad_fn<float>(vec)
+                   : dtype == DGN_F16 ? combine_grad_fn<__half>(vec)
+                                      : combine_grad_fn<__nv_bfloat16>(vec);
+  DGN_ON(device);
+  void* args[] = {&p};
+  return launch(fn, dim3((unsigned)(tokens + experts)), dim3(256), 0, stream, args);
+}
+
+extern "C" int dgn_expert_update_bias(const float* bias, const int32_t* counts, float* out, int experts, float rate,
+                                      int device, void* stream) {
+  int rc = check_experts(experts);
+  if (rc != DGN_OK) return rc;
+  if (!bias || !counts || !out) return null_pointer("dgn_expert_update_bias: null pointer");
+  if (!aligned(bias, 4) || !aligned(counts, 4) || !aligned(out, 4)) return misaligned();
+  DGN_ON(device);
+  void* args[] = {&bias, &counts, &out, &experts, &rate};
+  return launch((const void*)update_bias_kernel, dim3(1), dim3(1024), 0, stream, args);
+}

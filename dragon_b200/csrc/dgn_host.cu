@@ -1469,6 +1469,9 @@ namespace dgn {
 // For the other translation units of the library: record an error message for
 // dgn_last_error_string and hand back `code`.
 int report_error(int code, const char* message) { return fail(code, "%s", message); }
+
+// One more kernel of this library was launched (dgn_launch_count).
+void count_launch() { g_launches.fetch_add(1); }
 }  // namespace dgn
 
 // Sets up the NVSwitch multicast staging if every rank can take part: all

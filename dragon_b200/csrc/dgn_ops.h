@@ -1,0 +1,53 @@
+// Host helpers shared by the single-GPU operators (dgn_norm.cu, dgn_experts.cu):
+// error reporting, launch accounting, the device switch and alignment tests.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/dgn.h"
+
+namespace dgn {
+
+int report_error(int code, const char* message);  // dgn_host.cu: sets dgn_last_error_string
+void count_launch();                               // dgn_host.cu: dgn_launch_count
+
+// Makes `device` current for one call and puts the caller's device back.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    err_ = cudaGetDevice(&prev_);
+    if (err_ == cudaSuccess && prev_ != device) {
+      err_ = cudaSetDevice(device);
+      switched_ = err_ == cudaSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (switched_) cudaSetDevice(prev_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  cudaError_t error() const { return err_; }
+
+ private:
+  int prev_ = -1;
+  bool switched_ = false;
+  cudaError_t err_;
+};
+
+// One launch of `fn` on `stream`; a failure is reported and cleared.
+inline int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* stream, void** args) {
+  cudaError_t e = cudaLaunchKernel(fn, grid, block, args, smem, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
+  }
+  count_launch();
+  return DGN_OK;
+}
+
+inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool float_dtype(int dtype) { return dtype == DGN_F16 || dtype == DGN_BF16 || dtype == DGN_F32; }
+
+}  // namespace dgn

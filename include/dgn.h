@@ -353,6 +353,113 @@ int dgn_allreduce_static(int nranks, const void* const* in_ptrs, void* const* ou
  * allocates nothing. */
 int dgn_allreduce_static_status(int clear);
 
+/* ---- norm and expert operators of a model's layers --------------------------
+ * Work of one GPU next to the collectives: the norm whose rows the all-gather
+ * moves (the normalisation operators of the reference end at the statistics
+ * exchange above; it has no root-mean-square norm), and the operators of a
+ * layer of experts, whose token counts the group adds up.  They need no
+ * communicator: `device` is the CUDA device that holds every pointer of the
+ * call and to which `stream` belongs (the caller's current device is put back),
+ * a call only enqueues kernels, allocates nothing and keeps nothing, and may be
+ * captured.  Matrices have contiguous rows; a `stride` counts elements from one
+ * row to the next.  Outputs must not overlap inputs except where said.
+ *
+ * dgn_rms_norm: hidden = x + residual (rounded to `dtype`; without a residual
+ * hidden is x itself and not written), rstd = 1/sqrt(mean(hidden^2) + eps),
+ * out = hidden * rstd * weight.  dtype: DGN_F16, DGN_BF16, DGN_F32; 1..32768
+ * columns.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
+ * be the residual's own memory with the same stride.  The sum of squares is
+ * held in float32.  With a code, out holds 8-bit values instead and scales one
+ * float32 per row and group of `group` columns (32, 64, 128, or 0: the row):
+ * value = code * scale, scale = largest magnitude / largest code (127, 448,
+ * 57344), groups below 2^-40 taking that bound's scale; a group with a NaN or an
+ * infinity has scale NaN.  out, scales [rows, groups] and rstd are contiguous. */
+typedef enum { DGN_CODE_NONE = 0, DGN_CODE_I8 = 1, DGN_CODE_E4M3 = 2, DGN_CODE_E5M2 = 3 } dgn_code;
+
+int dgn_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                 const void* weight, int weight_dtype, void* hidden, int64_t hidden_stride, void* out, int code,
+                 int64_t group, float* scales, float* rstd, int64_t rows, int64_t cols, float eps, int dtype,
+                 int device, void* stream);
+
+/* Backward pass: grad_x (contiguous) is the gradient of x and of the residual
+ * alike; grad_hidden, the gradient that reaches `hidden` by other ways, may be
+ * NULL; grad_weight (type weight_dtype, sums in float32 in a fixed order) may be
+ * NULL, otherwise `workspace` holds dgn_rms_norm_grad_workspace bytes.  grad_x
+ * may be grad_out's or grad_hidden's own memory if that is contiguous. */
+int64_t dgn_rms_norm_grad_workspace(int64_t rows, int64_t cols, int dtype);
+int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, const void* grad_hidden,
+                      int64_t grad_hidden_stride, const void* hidden, int64_t hidden_stride, const void* weight,
+                      int weight_dtype, const float* rstd, void* grad_x, void* grad_weight, void* workspace,
+                      int64_t workspace_bytes, int64_t rows, int64_t cols, int dtype, int device, void* stream);
+
+/* dgn_route: the k experts of each token and their weights.
+ *   score = softmax(logits) or sigmoid(logits);  key = logit, or score + bias
+ *   groups > 1: the experts lie in `groups` equal runs, and only those of the
+ *     `keep` best runs count; a run's value is the sum of its `best` (1 or 2)
+ *     largest keys (scores where there is no bias and best is 2)
+ *   the k largest keys, in falling order, equal ones by the lower index
+ *   weight = scale * score, or scale * score / (sum of the k scores + 1e-20)
+ * Choices are made as if computed in 64 bits, so that ranks and recomputations
+ * agree.  An expert whose logit or key is -inf is not chosen; a NaN counts as
+ * the largest key.  Slots that find no expert, and the tokens whose `mask` byte
+ * is 0, get index -1 and weight 0.  1..1024 experts, k 1..32 and at most the
+ * number of experts, 1..32 groups. */
+typedef enum { DGN_SCORE_SOFTMAX = 0, DGN_SCORE_SIGMOID = 1 } dgn_score;
+
+int dgn_route(const void* logits, int64_t stride, const float* bias, const uint8_t* mask, int32_t* indices,
+              float* weights, int64_t tokens, int experts, int k, int score, int groups, int keep, int best,
+              int renormalize, float scale, int dtype, int device, void* stream);
+
+/* Gradient of the logits (contiguous, type `dtype`) from that of the weights.
+ * Indices outside 0..experts-1 take no part; one that stands twice in a token's
+ * list counts twice. */
+int dgn_route_grad(const float* grad_weights, const void* logits, int64_t stride, const int32_t* indices,
+                   void* grad_logits, int64_t tokens, int experts, int k, int score, int renormalize, float scale,
+                   int dtype, int device, void* stream);
+
+/* dgn_expert_plan: where each of the `slots` = tokens * k (token, choice) pairs
+ * goes when rows are put in the order of their experts, equal ones in the order
+ * of the slots.  Expert e's rows start at offsets[e], a multiple of `align`;
+ * counts[e] of them are in use, offsets[e+1] begins the next block and
+ * offsets[experts] ends the last.  positions[slot] is -1 for an index outside
+ * 0..experts-1.  slots + min(experts, slots) * (align - 1) rows suffice (below
+ * 2^31).  `workspace`: dgn_expert_plan_workspace bytes (may be 0). */
+int64_t dgn_expert_plan_workspace(int64_t slots, int experts);
+int dgn_expert_plan(const int32_t* indices, int64_t slots, int experts, int align, int32_t* counts, int32_t* offsets,
+                    int32_t* positions, void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/* out[positions[t*k+j]] = x[t] for rows of row_bytes bytes (any type), x_stride
+ * bytes apart in x and contiguous in out, which has `capacity` rows.  The unused
+ * rows of each expert's block become zeros, rows behind the last block stay as
+ * they are.  A position outside 0..capacity-1 is passed over. */
+int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_bytes, const int32_t* positions,
+                        const int32_t* counts, const int32_t* offsets, void* out, int64_t tokens, int k, int experts,
+                        int64_t capacity, int device, void* stream);
+
+/* out[t] = residual[t] + sum over j of weights[t*k+j] * rows[positions[t*k+j]]:
+ * float32 sums in the order of j, the residual last, one rounding.  weights NULL:
+ * ones (the gradient of dgn_expert_dispatch); residual NULL: none.  out may be
+ * the residual's own memory if that is contiguous. */
+int dgn_expert_combine(const void* rows, const int32_t* positions, const float* weights, const void* residual,
+                       int64_t residual_stride, void* out, int64_t tokens, int k, int64_t cols, int64_t capacity,
+                       int dtype, int device, void* stream);
+
+/* Backward pass of dgn_expert_combine: grad_rows[position] = weight * grad_out[t]
+ * (unused and further rows as in dgn_expert_dispatch), grad_weights[t*k+j] =
+ * <grad_out[t], rows[position]>, 0 where there is no position.  A position must
+ * stand for one slot only. */
+int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_stride, const void* rows,
+                            const int32_t* positions, const float* weights, const int32_t* counts,
+                            const int32_t* offsets, void* grad_rows, float* grad_weights, int64_t tokens, int k,
+                            int experts, int64_t cols, int64_t capacity, int dtype, int device, void* stream);
+
+/* out[e] = bias[e] + rate * sign(mean(counts) - counts[e]): experts that had
+ * fewer tokens than the mean become easier to choose.  `counts` are the group's
+ * (an all-reduce of dgn_expert_plan's), the mean is compared exactly.  out may
+ * be bias. */
+int dgn_expert_update_bias(const float* bias, const int32_t* counts, float* out, int experts, float rate, int device,
+                           void* stream);
+
 /* ---- introspection for benchmarks and tests ------------------------------ */
 
 /* The variant and launch shape the library would choose for one collective on a
