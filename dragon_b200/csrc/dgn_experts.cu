@@ -736,10 +736,6 @@ extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int expert
     if (rc != DGN_OK) return rc;
   }
   const int smem = kPlanWarps * experts * (int)sizeof(int);
-  if (smem > 48 << 10) {
-    cudaError_t e = cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
-  }
   return launch((const void*)plan_place_kernel, dim3(blocks), dim3(kPlanThreads), smem, stream, args);
 }
 

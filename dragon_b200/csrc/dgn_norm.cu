@@ -23,8 +23,10 @@ namespace {
 using namespace dgn;
 
 constexpr int kMaxCols = 32768;
-constexpr int kMaxPartials = 592;         // rows of the weight gradient's partial sums: four blocks on each of 148 SMs
+constexpr int kSMs = 148;
+constexpr int kMaxPartials = 4 * kSMs;     // rows of the weight gradient's partial sums: four blocks on each SM at most
 constexpr float kSmallestAmax = 0x1p-40f;  // groups whose largest value is below this take this one's scale
+constexpr int kThreads = 256;              // of a block whose rows belong to teams of its threads
 
 struct NormParams {
   const char* x;
@@ -35,54 +37,70 @@ struct NormParams {
   float* scales;
   float* rstd;
   long long rows, x_stride, residual_stride, hidden_stride;  // strides in elements
-  int cols, group, groups;  // group: columns per scale; groups: scales per row
+  int cols, group_shift, groups;  // columns per scale as a power of two; scales per row
   int weight_f32, code;
   float eps;
 };
 
-// E consecutive elements from column c of a row, zeros behind the last column.
+// Threads and columns.  A row belongs to a team of `team` threads; each of them holds NV
+// parts of E elements (16 bytes).  Aligned rows (VEC): a part is one 16-byte vector, and
+// neighbouring threads have neighbouring vectors.  Other rows: neighbouring threads have
+// neighbouring elements, so that loads of one element each still fill whole lines.
 template <typename T, bool VEC>
-__device__ __forceinline__ uint4 load_part(const char* row, int c, int cols) {
-  if (VEC) return *reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T));
-  const T* p = reinterpret_cast<const T*>(row) + c;
+__device__ __forceinline__ int column(int i, int e, int thread, int team) {
+  return VEC ? (i * team + thread) * Elem<T>::E + e : (i * Elem<T>::E + e) * team + thread;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load_part(const char* row, int i, int thread, int team, int cols) {
+  if (VEC) {
+    const int c = column<T, VEC>(i, 0, thread, team);
+    return c < cols ? *reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T)) : make_uint4(0, 0, 0, 0);
+  }
   uint4 v = make_uint4(0, 0, 0, 0);
-  T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-  for (int i = 0; i < Elem<T>::E; ++i)
-    if (c + i < cols) e[i] = p[i];
+  for (int e = 0; e < Elem<T>::E; ++e) {
+    const int c = column<T, VEC>(i, e, thread, team);
+    if (c < cols) reinterpret_cast<T*>(&v)[e] = reinterpret_cast<const T*>(row)[c];
+  }
   return v;
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_part(char* row, int c, int cols, uint4 v) {
+__device__ __forceinline__ void store_part(char* row, int i, int thread, int team, int cols, uint4 v) {
   if (VEC) {
-    *reinterpret_cast<uint4*>(row + (size_t)c * sizeof(T)) = v;
+    const int c = column<T, VEC>(i, 0, thread, team);
+    if (c < cols) *reinterpret_cast<uint4*>(row + (size_t)c * sizeof(T)) = v;
     return;
   }
-  T* p = reinterpret_cast<T*>(row) + c;
-  const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-  for (int i = 0; i < Elem<T>::E; ++i)
-    if (c + i < cols) p[i] = e[i];
+  for (int e = 0; e < Elem<T>::E; ++e) {
+    const int c = column<T, VEC>(i, e, thread, team);
+    if (c < cols) reinterpret_cast<T*>(row)[c] = reinterpret_cast<const T*>(&v)[e];
+  }
 }
 
-// The weights of E columns in float32 (ones without a weight).
+// The weights of a part in float32: ones without a weight, zeros behind the last column.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight(const char* weight, int f32, int c, int cols, float* w) {
+__device__ __forceinline__ void load_weight(const char* weight, int f32, int i, int thread, int team, int cols, float* w) {
   constexpr int E = Elem<T>::E;
   if (!weight) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) w[i] = 1.f;
+    for (int e = 0; e < E; ++e) w[e] = 1.f;
   } else if (!f32) {
-    Elem<T>::unpack(load_part<T, VEC>(weight, c, cols), w);
+    Elem<T>::unpack(load_part<T, VEC>(weight, i, thread, team, cols), w);
   } else if (VEC) {
+    const int c = column<T, VEC>(i, 0, thread, team);
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(weight + (size_t)(c + i) * 4);
-      w[i] = f.x; w[i + 1] = f.y; w[i + 2] = f.z; w[i + 3] = f.w;
+    for (int e = 0; e < E; e += 4) {
+      const float4 f = c < cols ? *reinterpret_cast<const float4*>(weight + (size_t)(c + e) * 4) : make_float4(0, 0, 0, 0);
+      w[e] = f.x; w[e + 1] = f.y; w[e + 2] = f.z; w[e + 3] = f.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) w[i] = c + i < cols ? reinterpret_cast<const float*>(weight)[c + i] : 0.f;
+    for (int e = 0; e < E; ++e) {
+      const int c = column<T, VEC>(i, e, thread, team);
+      w[e] = c < cols ? reinterpret_cast<const float*>(weight)[c] : 0.f;
+    }
   }
 }
 
@@ -91,21 +109,25 @@ struct Sum { static __device__ float of(float a, float b) { return a + b; } };
 struct Largest { static __device__ float of(float a, float b) {
   return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
 
-// One value for all threads of a row: a warp's lanes, then its row's warps through
-// shared memory.  `slot` has 32 entries for each row of the block.
-template <typename Op>
-__device__ __forceinline__ float row_reduce(float v, float* slot) {
+// One value of each of RU rows for all threads of their team: TEAM lanes of a warp, or
+// (TEAM 0) the block, whose warps meet in `slot`.  A slot is written again only behind
+// another barrier of the caller's: two of them take turns.
+template <typename Op, int TEAM, int RU>
+__device__ __forceinline__ void team_reduce(float (&v)[RU], float* slot) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) v = Op::of(v, __shfl_xor_sync(0xffffffffu, v, d));
+  for (int d = (TEAM ? TEAM : 32) / 2; d; d >>= 1)
+#pragma unroll
+    for (int u = 0; u < RU; ++u) v[u] = Op::of(v[u], __shfl_xor_sync(0xffffffffu, v[u], d));
+  if (TEAM) return;
   const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v[0];
   __syncthreads();
-  v = (threadIdx.x & 31) < warps ? slot[threadIdx.x & 31] : 0.f;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v = Op::of(v, __shfl_xor_sync(0xffffffffu, v, d));
-  __syncthreads();
-  return v;
+  float all = 0.f;
+  for (int w = 0; w < warps; w += 4) {  // 32 slots, those of missing warps are zero
+    const float4 f = *reinterpret_cast<const float4*>(slot + w);
+    all = Op::of(all, Op::of(Op::of(f.x, f.y), Op::of(f.z, f.w)));
+  }
+  v[0] = all;
 }
 
 __device__ __forceinline__ unsigned encode2(float a, float b, int code) {
@@ -119,112 +141,177 @@ __device__ __forceinline__ float largest_code(int code) {
   return code == DGN_CODE_I8 ? 127.f : code == DGN_CODE_E4M3 ? 448.f : 57344.f;
 }
 
-// Threads (x, y): x works on row blockIdx.x * blockDim.y + y, which takes blockDim.x * NV * E >= cols columns.
-template <typename T, int NV, bool VEC, bool CODES>
-__global__ void __launch_bounds__(NV <= 2 ? 512 : 1024) rms_norm_kernel(const __grid_constant__ NormParams p) {
-  constexpr int E = Elem<T>::E;
-  __shared__ float slot[32];
-  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;  // rows share a block only when each has one warp: nobody waits for this one
-  const char* x = p.x + row * p.x_stride * (long long)sizeof(T);
-  const char* r = p.residual ? p.residual + row * p.residual_stride * (long long)sizeof(T) : nullptr;
-  char* hidden = r ? p.hidden + row * p.hidden_stride * (long long)sizeof(T) : nullptr;
-  uint4 h[NV];
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * E;
-    h[i] = make_uint4(0, 0, 0, 0);
-    if (c < p.cols) {
-      h[i] = load_part<T, VEC>(x, c, p.cols);
-      if (r) {
-        float a[E], b[E];
-        Elem<T>::unpack(h[i], a);
-        Elem<T>::unpack(load_part<T, VEC>(r, c, p.cols), b);
-#pragma unroll
-        for (int e = 0; e < E; ++e) a[e] += b[e];
-        h[i] = Elem<T>::pack(a);
-        store_part<T, VEC>(hidden, c, p.cols, h[i]);
-      }
-    }
-    float a[E];
-    Elem<T>::unpack(h[i], a);
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum = fmaf(a[e], a[e], sum);
+// Codes of values h * w * rstd from u = h * w alone: with m the largest |u| of the group, code = rn(u * (L / m)) and
+// scale = m * rstd / L, so that rstd's rounding does not move a code.  Returns the factor and sets the scale.
+__device__ __forceinline__ float code_factor(float m, float rstd, float largest, float* scale) {
+  const float nan = __uint_as_float(0x7fffffffu), top = m * rstd;
+  if (!(top < __uint_as_float(0x7f800000u))) {  // a NaN or an infinity: the group reads as NaN
+    *scale = nan;
+    return nan;
   }
-  sum = row_reduce<Sum>(sum, slot);
-  const float rstd = 1.f / sqrtf(sum / (float)p.cols + p.eps);
-  if (threadIdx.x == 0) p.rstd[row] = rstd;
+  *scale = fmaxf(top, kSmallestAmax) / largest;
+  return top >= kSmallestAmax ? largest / m : largest * rstd / kSmallestAmax;
+}
 
-  if (!CODES) {
-    char* out = p.out + row * p.cols * (long long)sizeof(T);
+// One row for a block (TEAM 0), or RU rows for a team of TEAM lanes; rows that are read
+// together lie next to each other.
+template <typename T, int TEAM, int NV, bool VEC, bool CODES>
+__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
+    rms_norm_kernel(const __grid_constant__ NormParams p) {
+  constexpr int E = Elem<T>::E, RU = !TEAM || !VEC ? 1 : NV == 1 ? 4 : NV == 2 ? 2 : 1;
+  constexpr long long S = sizeof(T);
+  __shared__ __align__(16) float slot[2][32];
+  __shared__ unsigned chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
+  const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
+  const long long first = (long long)blockIdx.x * blockDim.y * RU + threadIdx.y;
+  if (!TEAM) {
+    if (me < 64) slot[me >> 5][me & 31] = 0.f;
+    __syncthreads();
+  }
+  uint4 h[RU][NV], r[RU][NV];
+#pragma unroll
+  for (int u = 0; u < RU; ++u) {
+    const long long row = first + u * blockDim.y;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-      if (c >= p.cols) break;
-      float a[E], w[E];
-      Elem<T>::unpack(h[i], a);
-      load_weight<T, VEC>(p.weight, p.weight_f32, c, p.cols, w);
+      h[u][i] = r[u][i] = make_uint4(0, 0, 0, 0);
+      if (row < p.rows) {
+        h[u][i] = load_part<T, VEC>(p.x + row * p.x_stride * S, i, me, team, cols);
+        if (p.residual) r[u][i] = load_part<T, VEC>(p.residual + row * p.residual_stride * S, i, me, team, cols);
+      }
+    }
+  }
+  float sum[RU], rstd[RU];
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = a[e] * rstd * w[e];
-      store_part<T, VEC>(out, c, p.cols, Elem<T>::pack(a));
+  for (int u = 0; u < RU; ++u) {
+    const long long row = first + u * blockDim.y;
+    sum[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float a[E];
+      Elem<T>::unpack(h[u][i], a);
+      if (p.residual) {
+        float b[E];
+        Elem<T>::unpack(r[u][i], b);
+#pragma unroll
+        for (int e = 0; e < E; ++e) a[e] += b[e];
+        h[u][i] = Elem<T>::pack(a);
+        Elem<T>::unpack(h[u][i], a);
+        if (row < p.rows) store_part<T, VEC>(p.hidden + row * p.hidden_stride * S, i, me, team, cols, h[u][i]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[u] = fmaf(a[e], a[e], sum[u]);
+    }
+  }
+  team_reduce<Sum, TEAM>(sum, slot[0]);
+#pragma unroll
+  for (int u = 0; u < RU; ++u) {
+    const long long row = first + u * blockDim.y;
+    rstd[u] = 1.f / sqrtf(sum[u] / (float)cols + p.eps);
+    if (me == 0 && row < p.rows) p.rstd[row] = rstd[u];
+  }
+
+  if (!CODES) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float w[E];
+      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        const long long row = first + u * blockDim.y;
+        float a[E];
+        Elem<T>::unpack(h[u][i], a);
+#pragma unroll
+        for (int e = 0; e < E; ++e) a[e] = a[e] * rstd[u] * w[e];
+        if (row < p.rows) store_part<T, VEC>(p.out + row * cols * S, i, me, team, cols, Elem<T>::pack(a));
+      }
     }
     return;
   }
 
-  // 8-bit codes.  A group of at most 128 columns lies in the lanes of one warp (E = 4: 32 lanes); a scale per row
-  // takes one more reduction over the row.
+  // 8-bit codes.  Aligned rows: a group of at most 128 columns lies in neighbouring lanes of one warp.  Other rows: 32
+  // columns lie in the lanes of a warp, and larger groups are put together in shared memory.
   const float largest = largest_code(p.code);
-  unsigned char* out = reinterpret_cast<unsigned char*>(p.out) + row * p.cols;
-  float whole = 0.f;
-  if (p.groups == 1) {
+  const bool whole = p.groups == 1;
+  float top[RU];
+  if (whole || !VEC) {
+#pragma unroll
+    for (int u = 0; u < RU; ++u) top[u] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-      if (c >= p.cols) break;
-      float a[E], w[E];
-      Elem<T>::unpack(h[i], a);
-      load_weight<T, VEC>(p.weight, p.weight_f32, c, p.cols, w);
+      float w[E];
+      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) whole = Largest::of(whole, fabsf(a[e] * rstd * w[e]));
+      for (int u = 0; u < RU; ++u) {
+        float a[E];
+        Elem<T>::unpack(h[u][i], a);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float m = fabsf(a[e] * w[e]);
+          top[u] = Largest::of(top[u], m);
+          if (!VEC && !whole) {
+            const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            const int at = column<T, VEC>(i, e, me, team) >> 5;
+            if ((me & 31) == 0 && at * 32 < cols) chunk[threadIdx.y * 32 + at] = bits;
+          }
+        }
+      }
     }
-    whole = row_reduce<Largest>(whole, slot);
+    if (whole) team_reduce<Largest, TEAM>(top, slot[1]);
+    else if (TEAM) __syncwarp();
+    else __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * E;
-    float a[E], w[E], amax = 0.f;
-    Elem<T>::unpack(h[i], a);
-    if (c < p.cols) {
-      load_weight<T, VEC>(p.weight, p.weight_f32, c, p.cols, w);
+    float w[E];
+    load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        a[e] = a[e] * rstd * w[e];
-        if (VEC || c + e < p.cols) amax = Largest::of(amax, fabsf(a[e]));
+    for (int u = 0; u < RU; ++u) {
+      const long long row = first + u * blockDim.y;
+      unsigned char* out = reinterpret_cast<unsigned char*>(p.out) + row * cols;
+      float a[E], scale;
+      Elem<T>::unpack(h[u][i], a);
+#pragma unroll
+      for (int e = 0; e < E; ++e) a[e] *= w[e];
+      if (VEC) {
+        const int c = column<T, VEC>(i, 0, me, team);
+        float m = 0.f;
+        if (whole) {
+          m = top[u];
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) m = Largest::of(m, fabsf(a[e]));
+          for (int d = (1 << p.group_shift) / E / 2; d; d >>= 1) m = Largest::of(m, __shfl_xor_sync(0xffffffffu, m, d));
+        }
+        if (c >= cols || row >= p.rows) continue;
+        const float f = code_factor(m, rstd[u], largest, &scale);
+        if (whole ? c == 0 : (c & ((1 << p.group_shift) - 1)) == 0)
+          p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = scale;
+        unsigned code[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) code[e / 2] = encode2(a[e] * f, a[e + 1] * f, p.code);
+        const unsigned lo = code[0] | code[1] << 16;
+        if (E == 8) *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, code[E / 2 - 2] | code[E / 2 - 1] << 16);
+        else *reinterpret_cast<unsigned*>(out + c) = lo;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int c = column<T, VEC>(i, e, me, team);
+          if (c >= cols || row >= p.rows) continue;
+          float m = top[u];
+          int group = 0;
+          if (!whole) {
+            group = c >> p.group_shift;
+            const int begin = group << (p.group_shift - 5), end = min(begin + (1 << (p.group_shift - 5)), (cols + 31) >> 5);
+            unsigned bits = 0;
+            for (int k = begin; k < end; ++k) bits = max(bits, chunk[threadIdx.y * 32 + k]);
+            m = __uint_as_float(bits);
+          }
+          const float f = code_factor(m, rstd[u], largest, &scale);
+          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = scale;
+          out[c] = (unsigned char)encode2(a[e] * f, 0.f, p.code);
+        }
       }
-    }
-    if (p.groups == 1) {
-      amax = whole;
-    } else {
-      for (int d = p.group / E / 2; d; d >>= 1) amax = Largest::of(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    }
-    if (c >= p.cols) continue;
-    // A group with a NaN or an infinity has no scale: it reads as NaN.
-    const bool finite = __float_as_uint(amax) < 0x7f800000u;
-    const float top = fmaxf(amax, kSmallestAmax);
-    const float inv = finite ? largest / top : __uint_as_float(0x7fffffffu);
-    if (c % p.group == 0) p.scales[row * p.groups + c / p.group] = finite ? top / largest : __uint_as_float(0x7fffffffu);
-    unsigned code[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) code[e / 2] = encode2(a[e] * inv, a[e + 1] * inv, p.code);
-    if (VEC) {
-      const unsigned lo = code[0] | code[1] << 16;
-      if (E == 8) *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, code[E / 2 - 2] | code[E / 2 - 1] << 16);
-      else *reinterpret_cast<unsigned*>(out + c) = lo;
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (c + e < p.cols) out[c + e] = (unsigned char)(code[e / 2] >> (8 * (e & 1)));
     }
   }
 }
@@ -241,93 +328,209 @@ struct NormGradParams {
   int cols, weight_f32;
 };
 
-// Threads as above; a block takes every gridDim.x-th row (or set of blockDim.y rows) and keeps the weight gradient of
-// its rows in registers, so that the partial sums are as many as the blocks and their order is fixed.
-template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(NV <= 2 ? 512 : 1024) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+// Writes a block's sums of the weight gradient to its row of the partial sums; teams that
+// share the block are added in shared memory, in their order.
+template <typename T, int TEAM, int NV, bool VEC>
+__device__ __forceinline__ void store_partial(const NormGradParams& p, const float* acc, float* shared) {
   constexpr int E = Elem<T>::E;
-  extern __shared__ float shared[];  // several rows a block: blockDim.y * cols floats
-  __shared__ float slot[32];
+  const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
+  float* mine = p.partial + (long long)blockIdx.x * cols;
+  float* to = TEAM ? shared + threadIdx.y * cols : mine;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = column<T, VEC>(i, 0, me, team);
+    if (VEC && c < cols) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(to + c + e) = make_float4(acc[i * E + e], acc[i * E + e + 1], acc[i * E + e + 2], acc[i * E + e + 3]);
+    } else if (!VEC) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (column<T, VEC>(i, e, me, team) < cols) to[column<T, VEC>(i, e, me, team)] = acc[i * E + e];
+    }
+  }
+  if (!TEAM) return;
+  __syncthreads();
+  for (int c = threadIdx.y * TEAM + me; c < cols; c += kThreads) {
+    float s = 0.f;
+    for (int y = 0; y < (int)blockDim.y; ++y) s += shared[y * cols + c];
+    mine[c] = s;
+  }
+}
+
+// The plain form: rows straight into registers.  Taken by rows that are not aligned, by
+// short ones (a team of 8 or 16 lanes, four rows at a time) and by those too long for the ring below.
+template <typename T, int TEAM, int NV, bool VEC>
+__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
+    rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+  constexpr int E = Elem<T>::E, RU = TEAM && VEC ? 4 : 1;
+  constexpr long long S = sizeof(T);
+  extern __shared__ __align__(16) float shared[];  // teams * cols floats
+  __shared__ __align__(16) float slot[2][32];
+  const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
+  if (!TEAM) {
+    if (me < 64) slot[me >> 5][me & 31] = 0.f;
+    __syncthreads();
+  }
   float acc[NV * E];
 #pragma unroll
   for (int i = 0; i < NV * E; ++i) acc[i] = 0.f;
-  for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows;
-       row += (long long)gridDim.x * blockDim.y) {
-    const char* gp = p.grad_out + row * p.grad_out_stride * (long long)sizeof(T);
-    const char* hp = p.hidden + row * p.hidden_stride * (long long)sizeof(T);
-    const char* rp = p.grad_hidden ? p.grad_hidden + row * p.grad_hidden_stride * (long long)sizeof(T) : nullptr;
-    const float rstd = p.rstd[row];
-    uint4 g[NV], h[NV];
-    float dot = 0.f;
+  int turn = 0;
+  for (long long base = (long long)blockIdx.x * blockDim.y * RU; base < p.rows;
+       base += (long long)gridDim.x * blockDim.y * RU, turn ^= 1) {
+    uint4 g[RU][NV], h[RU][NV], r[RU][NV];
+    float dot[RU], rstd[RU];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-      g[i] = h[i] = make_uint4(0, 0, 0, 0);
-      if (c < p.cols) {
-        g[i] = load_part<T, VEC>(gp, c, p.cols);
-        h[i] = load_part<T, VEC>(hp, c, p.cols);
+    for (int u = 0; u < RU; ++u) {
+      const long long row = base + u * blockDim.y + threadIdx.y;
+      rstd[u] = row < p.rows ? p.rstd[row] : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        g[u][i] = h[u][i] = r[u][i] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows) {
+          g[u][i] = load_part<T, VEC>(p.grad_out + row * p.grad_out_stride * S, i, me, team, cols);
+          h[u][i] = load_part<T, VEC>(p.hidden + row * p.hidden_stride * S, i, me, team, cols);
+          if (p.grad_hidden) r[u][i] = load_part<T, VEC>(p.grad_hidden + row * p.grad_hidden_stride * S, i, me, team, cols);
+        }
       }
+      dot[u] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-      if (c >= p.cols) break;
-      float a[E], b[E], w[E];
+      float w[E];
+      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        float a[E], b[E];
+        Elem<T>::unpack(g[u][i], a);
+        Elem<T>::unpack(h[u][i], b);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float n = b[e] * rstd[u];
+          dot[u] = fmaf(a[e] * w[e], n, dot[u]);
+          acc[i * E + e] = fmaf(a[e], n, acc[i * E + e]);
+        }
+      }
+    }
+    team_reduce<Sum, TEAM>(dot, slot[turn]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float w[E];
+      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+#pragma unroll
+      for (int u = 0; u < RU; ++u) {
+        const long long row = base + u * blockDim.y + threadIdx.y;
+        const float mean = dot[u] / (float)cols;
+        float a[E], b[E], c[E];
+        Elem<T>::unpack(g[u][i], a);
+        Elem<T>::unpack(h[u][i], b);
+        Elem<T>::unpack(r[u][i], c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) a[e] = rstd[u] * (a[e] * w[e] - b[e] * rstd[u] * mean) + c[e];
+        if (row < p.rows) store_part<T, VEC>(p.grad_x + row * cols * S, i, me, team, cols, Elem<T>::pack(a));
+      }
+    }
+  }
+  if (p.partial) store_partial<T, TEAM, NV, VEC>(p, acc, shared);
+}
+
+__device__ __forceinline__ void copy_async(uint4* to, const char* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+// Aligned rows.  Each thread copies its own vectors of the rows to come into its own places of a ring in shared memory
+// (cp.async), so the loads of STAGES - 1 rows are in flight while one is worked on and nobody waits for another
+// thread's copy; the sums of the weight gradient (and up to 16 weights a thread) stay in
+// registers for all of the block's rows.
+template <typename T, int TEAM, int NV, bool RESIDUAL>
+__global__ void __launch_bounds__(TEAM ? kThreads : 512) rms_norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
+  constexpr int E = Elem<T>::E, STAGES = NV == 4 ? 2 : 4, TENSORS = RESIDUAL ? 3 : 2;
+  constexpr long long S = sizeof(T);
+  extern __shared__ __align__(16) uint4 ring[];  // [STAGES][TENSORS][NV][threads]
+  __shared__ __align__(16) float slot[2][32];
+  const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
+  const int threads = blockDim.x * blockDim.y, place = threadIdx.y * blockDim.x + me;
+  if (!TEAM) {
+    for (int i = me; i < 64; i += blockDim.x) slot[i >> 5][i & 31] = 0.f;
+    __syncthreads();
+  }
+  const long long step = (long long)gridDim.x * blockDim.y;
+  auto fetch = [&](int stage, long long row) {
+    uint4* to = ring + (size_t)stage * TENSORS * NV * threads + place;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = column<T, true>(i, 0, me, team);
+      if (row < p.rows && c < cols) {
+        copy_async(to + (0 * NV + i) * threads, p.grad_out + (row * p.grad_out_stride + c) * S);
+        copy_async(to + (1 * NV + i) * threads, p.hidden + (row * p.hidden_stride + c) * S);
+        if (RESIDUAL) copy_async(to + (2 * NV + i) * threads, p.grad_hidden + (row * p.grad_hidden_stride + c) * S);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch(s, row + s * step);
+  constexpr bool KEEP = NV * E <= 16;  // the weights in registers; more of them are read again for each row
+  float w[KEEP ? NV * E : E], acc[NV * E];
+  if (KEEP) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, w + i * E);
+  }
+#pragma unroll
+  for (int i = 0; i < NV * E; ++i) acc[i] = 0.f;
+  int stage = 0, turn = 0;
+  for (; row < p.rows; row += step, turn ^= 1) {
+    const float rstd = p.rstd[row];
+    // The stage that the previous row has left.
+    fetch(stage == 0 ? STAGES - 1 : stage - 1, row + (STAGES - 1) * step);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    const uint4* from = ring + (size_t)stage * TENSORS * NV * threads + place;
+    uint4 g[NV], h[NV];
+    float dot[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      g[i] = h[i] = make_uint4(0, 0, 0, 0);
+      if (column<T, true>(i, 0, me, team) < cols) {
+        g[i] = from[(0 * NV + i) * threads];
+        h[i] = from[(1 * NV + i) * threads];
+      }
+      float a[E], b[E], *wi = w + (KEEP ? i * E : 0);
+      if (!KEEP) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
       Elem<T>::unpack(g[i], a);
       Elem<T>::unpack(h[i], b);
-      load_weight<T, VEC>(p.weight, p.weight_f32, c, p.cols, w);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float n = b[e] * rstd;
-        dot = fmaf(a[e] * w[e], n, dot);
+        dot[0] = fmaf(a[e] * wi[e], n, dot[0]);
         acc[i * E + e] = fmaf(a[e], n, acc[i * E + e]);
       }
     }
-    dot = row_reduce<Sum>(dot, slot) / (float)p.cols;
-    char* out = p.grad_x + row * p.cols * (long long)sizeof(T);
+    team_reduce<Sum, TEAM>(dot, slot[turn]);
+    const float mean = dot[0] / (float)cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-      if (c >= p.cols) break;
-      float a[E], b[E], w[E];
+      const int c = column<T, true>(i, 0, me, team);
+      if (c >= cols) continue;
+      float a[E], b[E], *wi = w + (KEEP ? i * E : 0);
+      if (!KEEP) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
       Elem<T>::unpack(g[i], a);
       Elem<T>::unpack(h[i], b);
-      load_weight<T, VEC>(p.weight, p.weight_f32, c, p.cols, w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = rstd * (a[e] * w[e] - b[e] * rstd * dot);
-      if (rp) {
-        Elem<T>::unpack(load_part<T, VEC>(rp, c, p.cols), b);
+      for (int e = 0; e < E; ++e) a[e] = rstd * (a[e] * wi[e] - b[e] * rstd * mean);
+      if (RESIDUAL) {
+        Elem<T>::unpack(from[(2 * NV + i) * threads], b);
 #pragma unroll
         for (int e = 0; e < E; ++e) a[e] += b[e];
       }
-      store_part<T, VEC>(out, c, p.cols, Elem<T>::pack(a));
+      *reinterpret_cast<uint4*>(p.grad_x + (row * cols + c) * S) = Elem<T>::pack(a);
     }
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (!p.partial) return;
-  float* mine = p.partial + (long long)blockIdx.x * p.cols;
-  if (blockDim.y == 1) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * blockDim.x + threadIdx.x) * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (c + e < p.cols) mine[c + e] = acc[i * E + e];
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (c + e < p.cols) shared[threadIdx.y * p.cols + c + e] = acc[i * E + e];
-  }
-  __syncthreads();
-  for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < p.cols; c += blockDim.x * blockDim.y) {
-    float s = 0.f;
-    for (int y = 0; y < (int)blockDim.y; ++y) s += shared[y * p.cols + c];
-    mine[c] = s;
-  }
+  if (TEAM) __syncthreads();  // the ring becomes the teams' meeting place
+  store_partial<T, TEAM, NV, true>(p, acc, reinterpret_cast<float*>(ring));
 }
 
 // Sum of the partial rows: a block of 32 x 32 threads takes 32 columns, a warp every 32nd partial row.
@@ -347,66 +550,93 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* par
   if (threadIdx.x == 0 && o < cols) grad[o] = W(v);
 }
 
-// Launch shape of a row kernel: `threads` for a row, `vectors` for a thread, `rows` for a block.
+// Launch shape of a row kernel: a team of `team` threads with `vectors` parts each, `teams` of them in a block.
 struct RowShape {
-  int threads, vectors, rows;
+  int team, vectors, teams;
+  int lanes() const { return teams > 1 ? team : 0; }  // the kernels' TEAM
 };
-RowShape row_shape(int64_t rows, int cols, int elems) {
-  const int nvec = (int)ceil_div(cols, elems);
-  RowShape s;
-  s.rows = 1;
-  if (nvec <= 128) {  // a warp for a row needs no barrier
-    s.threads = 32;
-    s.vectors = nvec <= 32 ? 1 : nvec <= 64 ? 2 : 4;
-    s.rows = 4;
-    return s;
+
+// Rows of up to 128 parts go to a warp or a half or quarter of one and need no barrier; longer ones to a block, with
+// more parts for a thread where the threads would pass 512.
+RowShape row_shape(int cols, int elems, bool vec) {
+  const int parts = (int)ceil_div(cols, elems);
+  if (parts <= 128) {
+    const int team = !vec ? 32 : parts <= 8 ? 8 : parts <= 16 ? 16 : 32;
+    return {team, parts <= 32 ? 1 : parts <= 64 ? 2 : 4, kThreads / team};
   }
-  s.vectors = nvec <= 1024 ? 2 : nvec <= 4096 ? 4 : 8;
-  s.threads = (int)ceil_div(ceil_div(nvec, s.vectors), 32) * 32;
-  return s;
+  const int vectors = parts <= 512 ? 2 : parts <= 4096 ? 4 : 8;
+  return {(int)ceil_div(ceil_div(parts, vectors), 32) * 32, vectors, 1};
 }
 
 template <typename T, bool VEC, bool CODES>
-const void* norm_kernel_nv(int nv) {
-  switch (nv) {
-    case 1: return (const void*)rms_norm_kernel<T, 1, VEC, CODES>;
-    case 2: return (const void*)rms_norm_kernel<T, 2, VEC, CODES>;
-    case 4: return (const void*)rms_norm_kernel<T, 4, VEC, CODES>;
-    default: break;
+const void* norm_kernel_of(const RowShape& s) {
+  if constexpr (VEC) {
+    if (s.lanes() == 8) return (const void*)rms_norm_kernel<T, 8, 1, VEC, CODES>;
+    if (s.lanes() == 16) return (const void*)rms_norm_kernel<T, 16, 1, VEC, CODES>;
   }
-  if constexpr (Elem<T>::E == 4) {  // more than 4096 vectors a row: float32 only
-    return (const void*)rms_norm_kernel<T, 8, VEC, CODES>;
-  } else {
-    return nullptr;
+  if (s.lanes() == 32) {
+    if (s.vectors == 1) return (const void*)rms_norm_kernel<T, 32, 1, VEC, CODES>;
+    if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 32, 2, VEC, CODES>;
+    return (const void*)rms_norm_kernel<T, 32, 4, VEC, CODES>;
   }
+  if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 0, 2, VEC, CODES>;
+  if constexpr (Elem<T>::E == 4)  // more than 4096 parts: float32 only
+    if (s.vectors == 8) return (const void*)rms_norm_kernel<T, 0, 8, VEC, CODES>;
+  return (const void*)rms_norm_kernel<T, 0, 4, VEC, CODES>;
 }
 template <typename T>
-const void* norm_kernel(int nv, bool vec, bool codes) {
-  if (vec) return codes ? norm_kernel_nv<T, true, true>(nv) : norm_kernel_nv<T, true, false>(nv);
-  return codes ? norm_kernel_nv<T, false, true>(nv) : norm_kernel_nv<T, false, false>(nv);
-}
-template <typename T, bool VEC>
-const void* norm_grad_kernel_nv(int nv) {
-  switch (nv) {
-    case 1: return (const void*)rms_norm_grad_kernel<T, 1, VEC>;
-    case 2: return (const void*)rms_norm_grad_kernel<T, 2, VEC>;
-    case 4: return (const void*)rms_norm_grad_kernel<T, 4, VEC>;
-    default: break;
-  }
-  if constexpr (Elem<T>::E == 4) {
-    return (const void*)rms_norm_grad_kernel<T, 8, VEC>;
-  } else {
-    return nullptr;
-  }
-}
-template <typename T>
-const void* norm_grad_kernel(int nv, bool vec) {
-  return vec ? norm_grad_kernel_nv<T, true>(nv) : norm_grad_kernel_nv<T, false>(nv);
+const void* norm_kernel(const RowShape& s, bool vec, bool codes) {
+  if (vec) return codes ? norm_kernel_of<T, true, true>(s) : norm_kernel_of<T, true, false>(s);
+  return codes ? norm_kernel_of<T, false, true>(s) : norm_kernel_of<T, false, false>(s);
 }
 
-int partial_rows(int64_t rows, const RowShape& s) {
-  const int64_t sets = ceil_div(rows, s.rows);
-  return (int)(sets < kMaxPartials ? sets : kMaxPartials);
+// Whether the ring takes a row: aligned, more than 16 parts, and two stages of 512 threads' parts are enough.
+bool ring_takes(const RowShape& s, bool vec) { return vec && s.team > 16 && s.team <= 512; }
+
+template <typename T, bool VEC>
+const void* norm_grad_kernel_of(const RowShape& s) {
+  if constexpr (VEC) {
+    if (s.lanes() == 8) return (const void*)rms_norm_grad_kernel<T, 8, 1, VEC>;
+    if (s.lanes() == 16) return (const void*)rms_norm_grad_kernel<T, 16, 1, VEC>;
+  } else {
+    if (s.lanes() == 32) {
+      if (s.vectors == 1) return (const void*)rms_norm_grad_kernel<T, 32, 1, VEC>;
+      if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 32, 2, VEC>;
+      return (const void*)rms_norm_grad_kernel<T, 32, 4, VEC>;
+    }
+    if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 0, 2, VEC>;
+  }
+  if constexpr (Elem<T>::E == 4)
+    if (s.vectors == 8) return (const void*)rms_norm_grad_kernel<T, 0, 8, VEC>;
+  return (const void*)rms_norm_grad_kernel<T, 0, 4, VEC>;
+}
+template <typename T, bool RESIDUAL>
+const void* norm_grad_ring_of(const RowShape& s) {
+  if (s.lanes() == 32) {
+    if (s.vectors == 1) return (const void*)rms_norm_grad_ring_kernel<T, 32, 1, RESIDUAL>;
+    if (s.vectors == 2) return (const void*)rms_norm_grad_ring_kernel<T, 32, 2, RESIDUAL>;
+    return (const void*)rms_norm_grad_ring_kernel<T, 32, 4, RESIDUAL>;
+  }
+  if (s.vectors == 2) return (const void*)rms_norm_grad_ring_kernel<T, 0, 2, RESIDUAL>;
+  return (const void*)rms_norm_grad_ring_kernel<T, 0, 4, RESIDUAL>;
+}
+template <typename T>
+const void* norm_grad_kernel(const RowShape& s, bool vec, bool residual) {
+  if (ring_takes(s, vec)) return residual ? norm_grad_ring_of<T, true>(s) : norm_grad_ring_of<T, false>(s);
+  return vec ? norm_grad_kernel_of<T, true>(s) : norm_grad_kernel_of<T, false>(s);
+}
+
+// Shared memory of a backward block.
+size_t grad_shared(const RowShape& s, bool vec, bool residual, int64_t cols) {
+  if (ring_takes(s, vec)) return (size_t)(s.vectors == 4 ? 2 : 4) * (residual ? 3 : 2) * s.vectors * s.team * s.teams * 16;
+  return s.teams > 1 ? (size_t)s.teams * cols * sizeof(float) : 0;
+}
+
+// Blocks of the backward pass: as many as fit an SM, four at most, and no more than there are rows for.
+int grad_blocks(const RowShape& s, size_t shared, int64_t rows) {
+  const int64_t fit = shared ? (int64_t)(220 << 10) / (int64_t)shared : 4;
+  const int64_t most = kSMs * (fit < 1 ? 1 : fit > 4 ? 4 : fit), sets = ceil_div(rows, s.teams);
+  return (int)(sets < most ? sets : most);
 }
 
 int check_matrix(int64_t rows, int64_t cols, int dtype) {
@@ -444,7 +674,7 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
                    (!weight || aligned(weight, 16)) &&
                    (!residual || (aligned(residual, 16) && aligned(hidden, 16) && residual_stride % elems == 0 &&
                                   hidden_stride % elems == 0));
-  const RowShape s = row_shape(rows, (int)cols, elems);
+  const RowShape s = row_shape((int)cols, elems, vec);
   NormParams p;
   p.x = static_cast<const char*>(x);
   p.residual = static_cast<const char*>(residual);
@@ -458,24 +688,26 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
   p.residual_stride = residual_stride;
   p.hidden_stride = hidden_stride;
   p.cols = (int)cols;
-  p.group = group && group < cols ? (int)group : (int)cols;
-  p.groups = (int)ceil_div(cols, p.group);
+  p.group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+  p.groups = group ? (int)ceil_div(cols, group) : 1;
   p.weight_f32 = weight_dtype == DGN_F32;
   p.code = code;
   p.eps = eps;
-  const void* fn = dtype == DGN_F32   ? norm_kernel<float>(s.vectors, vec, code != 0)
-                   : dtype == DGN_F16 ? norm_kernel<__half>(s.vectors, vec, code != 0)
-                                      : norm_kernel<__nv_bfloat16>(s.vectors, vec, code != 0);
+  const void* fn = dtype == DGN_F32   ? norm_kernel<float>(s, vec, code != 0)
+                   : dtype == DGN_F16 ? norm_kernel<__half>(s, vec, code != 0)
+                                      : norm_kernel<__nv_bfloat16>(s, vec, code != 0);
   OnDevice on(device);
   if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()));
+  // Rows of a block, as in the kernel: short aligned rows are taken four (one part) or two (two parts) at a time.
+  const int set = s.teams == 1 || !vec ? s.teams : s.teams * (s.vectors == 1 ? 4 : s.vectors == 2 ? 2 : 1);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)ceil_div(rows, s.rows)), dim3(s.threads, s.rows), 0, stream, args);
+  return launch(fn, dim3((unsigned)ceil_div(rows, set)), dim3(s.team, s.teams), 0, stream, args);
 }
 
 extern "C" int64_t dgn_rms_norm_grad_workspace(int64_t rows, int64_t cols, int dtype) {
   if (!float_dtype(dtype) || rows < 1 || cols < 1 || cols > kMaxCols) return 0;
-  const RowShape s = row_shape(rows, (int)cols, 16 / (int)dgn_dtype_size(dtype));
-  return (int64_t)partial_rows(rows, s) * cols * (int64_t)sizeof(float);
+  // Enough for either alignment of the rows: a block has one partial sum, and at least one row.
+  return (rows < kMaxPartials ? rows : kMaxPartials) * cols * (int64_t)sizeof(float);
 }
 
 extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, const void* grad_hidden,
@@ -506,13 +738,15 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   if (!aligned(grad_out, es) || !aligned(hidden, es) || !aligned(grad_hidden, es) || !aligned(grad_x, es) ||
       (weight && !aligned(weight, ws)) || !aligned(rstd, 4) || !aligned(workspace, 4))
     return report_error(DGN_ERR_ARG, "a pointer is not aligned to its element size");
-  const RowShape s = row_shape(rows, (int)cols, elems);
-  const int parts = partial_rows(rows, s);
-  if (grad_weight && workspace_bytes < (int64_t)parts * cols * (int64_t)sizeof(float))
-    return report_error(DGN_ERR_ARG, "dgn_rms_norm_grad: workspace too small");
   const bool vec = cols % elems == 0 && aligned(grad_out, 16) && grad_out_stride % elems == 0 && aligned(hidden, 16) &&
                    hidden_stride % elems == 0 && aligned(grad_x, 16) && (!weight || aligned(weight, 16)) &&
-                   (!grad_hidden || (aligned(grad_hidden, 16) && grad_hidden_stride % elems == 0));
+                   (!grad_hidden || (aligned(grad_hidden, 16) && grad_hidden_stride % elems == 0)) &&
+                   aligned(workspace, 16);
+  const RowShape s = row_shape((int)cols, elems, vec);
+  const size_t smem = grad_shared(s, vec, grad_hidden != nullptr, cols);
+  const int parts = grad_blocks(s, smem, rows);
+  if (grad_weight && workspace_bytes < (int64_t)parts * cols * (int64_t)sizeof(float))
+    return report_error(DGN_ERR_ARG, "dgn_rms_norm_grad: workspace too small");
   NormGradParams p;
   p.grad_out = static_cast<const char*>(grad_out);
   p.grad_hidden = static_cast<const char*>(grad_hidden);
@@ -527,12 +761,12 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   p.hidden_stride = hidden_stride;
   p.cols = (int)cols;
   p.weight_f32 = weight_dtype == DGN_F32;
-  const void* fn = dtype == DGN_F32   ? norm_grad_kernel<float>(s.vectors, vec)
-                   : dtype == DGN_F16 ? norm_grad_kernel<__half>(s.vectors, vec)
-                                      : norm_grad_kernel<__nv_bfloat16>(s.vectors, vec);
+  const bool residual = grad_hidden != nullptr;
+  const void* fn = dtype == DGN_F32   ? norm_grad_kernel<float>(s, vec, residual)
+                   : dtype == DGN_F16 ? norm_grad_kernel<__half>(s, vec, residual)
+                                      : norm_grad_kernel<__nv_bfloat16>(s, vec, residual);
   void* args[] = {&p};
-  const size_t smem = s.rows > 1 ? (size_t)s.rows * cols * sizeof(float) : 0;
-  rc = launch(fn, dim3(parts), dim3(s.threads, s.rows), smem, stream, args);
+  rc = launch(fn, dim3(parts), dim3(s.team, s.teams), smem, stream, args);
   if (rc != DGN_OK || !grad_weight) return rc;
   int nparts = parts, ncols = (int)cols;
   const float* partial = p.partial;

@@ -35,8 +35,20 @@ class OnDevice {
   cudaError_t err_;
 };
 
+// Lets `fn` be launched with `smem` bytes of dynamic shared memory.  Without this the
+// dynamic and the static part together may take 48 KiB; static parts here are below 8.
+inline int allow_shared(const void* fn, size_t smem) {
+  if (smem <= (40 << 10)) return DGN_OK;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) return DGN_OK;
+  cudaGetLastError();
+  return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
+}
+
 // One launch of `fn` on `stream`; a failure is reported and cleared.
 inline int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* stream, void** args) {
+  int rc = allow_shared(fn, smem);
+  if (rc != DGN_OK) return rc;
   cudaError_t e = cudaLaunchKernel(fn, grid, block, args, smem, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) {
     cudaGetLastError();

@@ -22,15 +22,11 @@ no autograd graph is recorded, the backward pass is the ``_grad`` calls.
 import torch
 
 from dragon_b200 import _C
-from dragon_b200.comm import _TORCH_TO_DGN, _enter_stream
+from dragon_b200.comm import _TORCH_TO_DGN, _enter_stream, _raw_stream
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _SCORES = {"softmax": _C.SCORE_SOFTMAX, "sigmoid": _C.SCORE_SIGMOID}
 MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 32
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _matrix(t, name, dtypes=_FLOATS):
@@ -118,7 +114,7 @@ def route(logits, k, bias=None, mask=None, scores="softmax", groups=1, keep_grou
         logits.data_ptr(), stride, bias.data_ptr() if bias is not None else None,
         mask.data_ptr() if mask is not None else None, indices.data_ptr(), weights.data_ptr(), tokens, experts, k, code,
         groups, keep_groups, group_best, bool(renormalize), scale, _TORCH_TO_DGN[logits.dtype], device.index,
-        _stream(device))
+        _raw_stream(device.index))
     if rc != _C.OK:
         _C.check(rc)
     return indices, weights
@@ -142,7 +138,7 @@ def route_grad(grad_weights, logits, indices, scores="softmax", renormalize=True
     grad = torch.empty((tokens, experts), dtype=logits.dtype, device=device)
     rc = _C.lib().dgn_route_grad(
         grad_weights.data_ptr(), logits.data_ptr(), stride, indices.data_ptr(), grad.data_ptr(), tokens, experts, k, code,
-        bool(renormalize), scale, _TORCH_TO_DGN[logits.dtype], device.index, _stream(device))
+        bool(renormalize), scale, _TORCH_TO_DGN[logits.dtype], device.index, _raw_stream(device.index))
     if rc != _C.OK:
         _C.check(rc)
     return grad
@@ -192,7 +188,7 @@ def plan(indices, num_experts, align=1, stream=None):
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     rc = lib.dgn_expert_plan(indices.data_ptr(), slots, num_experts, align, counts.data_ptr(), offsets.data_ptr(),
                              positions.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes, device.index,
-                             _stream(device))
+                             _raw_stream(device.index))
     if rc != _C.OK:
         _C.check(rc)
     return ExpertPlan(counts, offsets, positions, align)
@@ -235,7 +231,7 @@ def dispatch(x, plan, out=None, stream=None):
     rc = _C.lib().dgn_expert_dispatch(
         x.data_ptr(), stride * size, cols * size, plan.positions.data_ptr(), plan.counts.data_ptr(),
         plan.offsets.data_ptr(), out.data_ptr(), tokens, plan.k, plan.num_experts, out.shape[0], x.device.index,
-        _stream(x.device))
+        _raw_stream(x.device.index))
     if rc != _C.OK:
         _C.check(rc)
     return out
@@ -269,7 +265,7 @@ def combine(rows, plan, weights=None, residual=None, stream=None):
     rc = _C.lib().dgn_expert_combine(
         rows.data_ptr(), plan.positions.data_ptr(), weights.data_ptr() if weights is not None else None,
         residual.data_ptr() if residual is not None else None, residual_stride, out.data_ptr(), plan.tokens, plan.k, cols,
-        capacity, _TORCH_TO_DGN[rows.dtype], device.index, _stream(device))
+        capacity, _TORCH_TO_DGN[rows.dtype], device.index, _raw_stream(device.index))
     if rc != _C.OK:
         _C.check(rc)
     return out
@@ -308,7 +304,7 @@ def combine_grad(grad_output, rows, plan, weights, out=None, stream=None):
     rc = _C.lib().dgn_expert_combine_grad(
         grad_output.data_ptr(), stride, rows.data_ptr(), plan.positions.data_ptr(), weights.data_ptr(),
         plan.counts.data_ptr(), plan.offsets.data_ptr(), out.data_ptr(), grad_weights.data_ptr(), plan.tokens, plan.k,
-        plan.num_experts, cols, capacity, _TORCH_TO_DGN[rows.dtype], device.index, _stream(device))
+        plan.num_experts, cols, capacity, _TORCH_TO_DGN[rows.dtype], device.index, _raw_stream(device.index))
     if rc != _C.OK:
         _C.check(rc)
     return out, grad_weights
@@ -332,7 +328,7 @@ def update_bias(bias, counts, rate, out=None, stream=None):
         out = bias
     _exactly(out, "out", bias.device, bias.shape, (torch.float32,))
     rc = _C.lib().dgn_expert_update_bias(bias.data_ptr(), counts.data_ptr(), out.data_ptr(), bias.shape[0], rate,
-                                         bias.device.index, _stream(bias.device))
+                                         bias.device.index, _raw_stream(bias.device.index))
     if rc != _C.OK:
         _C.check(rc)
     return out

@@ -16,7 +16,7 @@ import collections
 import torch
 
 from dragon_b200 import _C
-from dragon_b200.comm import _TORCH_TO_DGN, _enter_stream
+from dragon_b200.comm import _TORCH_TO_DGN, _enter_stream, _raw_stream
 
 RMSNorm = collections.namedtuple("RMSNorm", ["output", "hidden", "rstd", "scale"])
 
@@ -129,7 +129,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, out_dtype=None, group_size
         weight.data_ptr() if weight is not None else None, weight_dtype,
         hidden.data_ptr() if residual is not None else None, hidden_stride, output.data_ptr(), code, group_size,
         scale.data_ptr() if code else None, rstd.data_ptr(), rows, cols, eps, dtype, x.device.index,
-        torch.cuda.current_stream(x.device).cuda_stream)
+        _raw_stream(x.device.index))
     if rc != _C.OK:
         _C.check(rc)
     return RMSNorm(output, hidden, rstd, scale)
@@ -171,7 +171,7 @@ def rms_norm_grad(grad_output, hidden, rstd, weight=None, grad_hidden=None, stre
         grad_hidden_stride, hidden.data_ptr(), hidden_stride, weight.data_ptr() if weight is not None else None,
         weight_dtype, rstd.data_ptr(), grad_x.data_ptr(), grad_weight.data_ptr() if weight is not None else None,
         workspace.data_ptr() if weight is not None else None, nbytes, rows, cols, dtype, hidden.device.index,
-        torch.cuda.current_stream(hidden.device).cuda_stream)
+        _raw_stream(hidden.device.index))
     if rc != _C.OK:
         _C.check(rc)
     return grad_x, grad_weight

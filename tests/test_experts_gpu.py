@@ -267,7 +267,7 @@ def choices(tokens, k, num, seed=0, missing=0.1):
 
 @pytest.mark.parametrize("tokens,k,num,align", [
     (0, 2, 4, 1), (1, 1, 1, 1), (1, 8, 256, 1), (3, 8, 256, 16), (31, 1, 7, 8), (100, 3, 5, 1), (513, 8, 64, 128),
-    (1365, 3, 33, 4), (1366, 3, 33, 4), (5000, 8, 1024, 1), (20000, 32, 300, 64), (70000, 10, 128, 1)])
+    (1365, 3, 33, 4), (1366, 3, 33, 4), (5000, 8, 1024, 1), (20000, 32, 300, 64), (70000, 10, 128, 1), (40, 8, 768, 1), (9000, 2, 768, 1)])
 def test_plan(dgn_lib, tokens, k, num, align):
     indices = choices(tokens, k, num)
     p = plan(indices, num, align)
