@@ -24,7 +24,7 @@ using namespace dgn;
 
 constexpr int kMaxCols = 32768;
 constexpr int kSMs = 148;
-constexpr int kMaxPartials = 4 * kSMs;     // rows of the weight gradient's partial sums: four blocks on each SM at most
+constexpr int kMaxPartials = 8 * kSMs;     // rows of the weight gradient's partial sums: eight blocks on each SM at most
 constexpr float kSmallestAmax = 0x1p-40f;  // groups whose largest value is below this take this one's scale
 constexpr int kThreads = 256;              // of a block whose rows belong to teams of its threads
 
@@ -104,10 +104,62 @@ __device__ __forceinline__ void load_weight(const char* weight, int f32, int i, 
   }
 }
 
+// Two float32 values in one instruction (add, mul and fma of f32x2, each rounded as the single one is).
+struct Pair {
+  u64 v;
+  __device__ Pair() {}
+  __device__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c.v) : "l"(a.v), "l"(b.v));
+  return c;
+}
+__device__ __forceinline__ Pair twice(float a) { return Pair(a, a); }
+
+// The E values of a part as pairs, and back.
+template <typename T> __device__ __forceinline__ void unpack2(uint4 v, Pair* a) {
+  float f[Elem<T>::E];
+  Elem<T>::unpack(v, f);
+#pragma unroll
+  for (int e = 0; e < Elem<T>::E; e += 2) a[e / 2] = Pair(f[e], f[e + 1]);
+}
+template <typename T> __device__ __forceinline__ uint4 pack2(const Pair* a) {
+  float f[Elem<T>::E];
+#pragma unroll
+  for (int e = 0; e < Elem<T>::E; e += 2) {
+    const float2 p = a[e / 2].get();
+    f[e] = p.x; f[e + 1] = p.y;
+  }
+  return Elem<T>::pack(f);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weight2(const char* weight, int f32, int i, int thread, int team, int cols, Pair* w) {
+  float f[Elem<T>::E];
+  load_weight<T, VEC>(weight, f32, i, thread, team, cols, f);
+#pragma unroll
+  for (int e = 0; e < Elem<T>::E; e += 2) w[e / 2] = Pair(f[e], f[e + 1]);
+}
+
 struct Sum { static __device__ float of(float a, float b) { return a + b; } };
-// Largest magnitude by the bits of |v|: NaN beats infinity beats every number.
+// The larger magnitude; a NaN stays one.
 struct Largest { static __device__ float of(float a, float b) {
-  return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return m;
+} };
 
 // One value of each of RU rows for all threads of their team: TEAM lanes of a warp, or
 // (TEAM 0) the block, whose warps meet in `slot`.  A slot is written again only behind
@@ -130,27 +182,43 @@ __device__ __forceinline__ void team_reduce(float (&v)[RU], float* slot) {
   v[0] = all;
 }
 
-__device__ __forceinline__ unsigned encode2(float a, float b, int code) {
+__device__ __forceinline__ unsigned encode1(float a, int code) {
+  if (code == DGN_CODE_I8) return (unsigned)min(max(__float2int_rn(a), -127), 127) & 255;  // NaN -> 0
+  return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, code == DGN_CODE_E4M3 ? __NV_E4M3 : __NV_E5M2);
+}
+// E codes, the first in the lowest byte.
+template <int E>
+__device__ __forceinline__ uint2 encode(const Pair* a, int code) {
+  unsigned w[4] = {0, 0, 0, 0};
   if (code == DGN_CODE_I8) {
-    const int i = min(max(__float2int_rn(a), -127), 127), j = min(max(__float2int_rn(b), -127), 127);  // NaN -> 0
-    return (unsigned)(i & 255) | (unsigned)(j & 255) << 8;
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      const float2 f = a[e].get();
+      w[e] = encode1(f.x, DGN_CODE_I8) | encode1(f.y, DGN_CODE_I8) << 8;
+    }
+  } else if (code == DGN_CODE_E4M3) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) w[e] = __nv_cvt_float2_to_fp8x2(a[e].get(), __NV_SATFINITE, __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) w[e] = __nv_cvt_float2_to_fp8x2(a[e].get(), __NV_SATFINITE, __NV_E5M2);
   }
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, code == DGN_CODE_E4M3 ? __NV_E4M3 : __NV_E5M2);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 __device__ __forceinline__ float largest_code(int code) {
   return code == DGN_CODE_I8 ? 127.f : code == DGN_CODE_E4M3 ? 448.f : 57344.f;
 }
 
 // Codes of values h * w * rstd from u = h * w alone: with m the largest |u| of the group, code = rn(u * (L / m)) and
-// scale = m * rstd / L, so that rstd's rounding does not move a code.  Returns the factor and sets the scale.
-__device__ __forceinline__ float code_factor(float m, float rstd, float largest, float* scale) {
-  const float nan = __uint_as_float(0x7fffffffu), top = m * rstd;
-  if (!(top < __uint_as_float(0x7f800000u))) {  // a NaN or an infinity: the group reads as NaN
-    *scale = nan;
-    return nan;
-  }
-  *scale = fmaxf(top, kSmallestAmax) / largest;
+// scale = m * rstd / L, so that rstd's rounding does not move a code.
+__device__ __forceinline__ float code_factor(float m, float rstd, float largest) {
+  const float top = m * rstd;
+  if (!(top < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);  // a NaN or an infinity: reads as NaN
   return top >= kSmallestAmax ? largest / m : largest * rstd / kSmallestAmax;
+}
+__device__ __forceinline__ float code_scale(float m, float rstd, float largest) {
+  const float top = m * rstd;
+  return top < __uint_as_float(0x7f800000u) ? fmaxf(top, kSmallestAmax) / largest : __uint_as_float(0x7fffffffu);
 }
 
 // One row for a block (TEAM 0), or RU rows for a team of TEAM lanes; rows that are read
@@ -185,23 +253,24 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
   for (int u = 0; u < RU; ++u) {
     const long long row = first + u * blockDim.y;
-    sum[u] = 0.f;
+    Pair squares(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float a[E];
-      Elem<T>::unpack(h[u][i], a);
+      Pair a[E / 2];
+      unpack2<T>(h[u][i], a);
       if (p.residual) {
-        float b[E];
-        Elem<T>::unpack(r[u][i], b);
+        Pair b[E / 2];
+        unpack2<T>(r[u][i], b);
 #pragma unroll
-        for (int e = 0; e < E; ++e) a[e] += b[e];
-        h[u][i] = Elem<T>::pack(a);
-        Elem<T>::unpack(h[u][i], a);
+        for (int e = 0; e < E / 2; ++e) a[e] = a[e] + b[e];
+        h[u][i] = pack2<T>(a);
+        if (sizeof(T) < 4) unpack2<T>(h[u][i], a);
         if (row < p.rows) store_part<T, VEC>(p.hidden + row * p.hidden_stride * S, i, me, team, cols, h[u][i]);
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum[u] = fmaf(a[e], a[e], sum[u]);
+      for (int e = 0; e < E / 2; ++e) squares = fma2(a[e], a[e], squares);
     }
+    sum[u] = squares.get().x + squares.get().y;
   }
   team_reduce<Sum, TEAM>(sum, slot[0]);
 #pragma unroll
@@ -214,16 +283,16 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
   if (!CODES) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float w[E];
-      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      Pair w[E / 2];
+      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         const long long row = first + u * blockDim.y;
-        float a[E];
-        Elem<T>::unpack(h[u][i], a);
+        Pair a[E / 2];
+        unpack2<T>(h[u][i], a);
 #pragma unroll
-        for (int e = 0; e < E; ++e) a[e] = a[e] * rstd[u] * w[e];
-        if (row < p.rows) store_part<T, VEC>(p.out + row * cols * S, i, me, team, cols, Elem<T>::pack(a));
+        for (int e = 0; e < E / 2; ++e) a[e] = a[e] * twice(rstd[u]) * w[e];
+        if (row < p.rows) store_part<T, VEC>(p.out + row * cols * S, i, me, team, cols, pack2<T>(a));
       }
     }
     return;
@@ -247,10 +316,10 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         Elem<T>::unpack(h[u][i], a);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float m = fabsf(a[e] * w[e]);
+          const float m = a[e] * w[e];
           top[u] = Largest::of(top[u], m);
           if (!VEC && !whole) {
-            const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(m)));  // by the bits a NaN is largest
             const int at = column<T, VEC>(i, e, me, team) >> 5;
             if ((me & 31) == 0 && at * 32 < cols) chunk[threadIdx.y * 32 + at] = bits;
           }
@@ -263,16 +332,16 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float w[E];
-    load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+    Pair w[E / 2];
+    load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
       const long long row = first + u * blockDim.y;
       unsigned char* out = reinterpret_cast<unsigned char*>(p.out) + row * cols;
-      float a[E], scale;
-      Elem<T>::unpack(h[u][i], a);
+      Pair a[E / 2];
+      unpack2<T>(h[u][i], a);
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] *= w[e];
+      for (int e = 0; e < E / 2; ++e) a[e] = a[e] * w[e];
       if (VEC) {
         const int c = column<T, VEC>(i, 0, me, team);
         float m = 0.f;
@@ -280,19 +349,18 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
           m = top[u];
         } else {
 #pragma unroll
-          for (int e = 0; e < E; ++e) m = Largest::of(m, fabsf(a[e]));
+          for (int e = 0; e < E / 2; ++e) m = Largest::of(m, Largest::of(a[e].get().x, a[e].get().y));
           for (int d = (1 << p.group_shift) / E / 2; d; d >>= 1) m = Largest::of(m, __shfl_xor_sync(0xffffffffu, m, d));
         }
         if (c >= cols || row >= p.rows) continue;
-        const float f = code_factor(m, rstd[u], largest, &scale);
         if (whole ? c == 0 : (c & ((1 << p.group_shift) - 1)) == 0)
-          p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = scale;
-        unsigned code[E / 2];
+          p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = code_scale(m, rstd[u], largest);
+        const Pair f = twice(code_factor(m, rstd[u], largest));
 #pragma unroll
-        for (int e = 0; e < E; e += 2) code[e / 2] = encode2(a[e] * f, a[e + 1] * f, p.code);
-        const unsigned lo = code[0] | code[1] << 16;
-        if (E == 8) *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, code[E / 2 - 2] | code[E / 2 - 1] << 16);
-        else *reinterpret_cast<unsigned*>(out + c) = lo;
+        for (int e = 0; e < E / 2; ++e) a[e] = a[e] * f;
+        const uint2 codes = encode<E>(a, p.code);
+        if (E == 8) *reinterpret_cast<uint2*>(out + c) = codes;
+        else *reinterpret_cast<unsigned*>(out + c) = codes.x;
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -307,9 +375,9 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
             for (int k = begin; k < end; ++k) bits = max(bits, chunk[threadIdx.y * 32 + k]);
             m = __uint_as_float(bits);
           }
-          const float f = code_factor(m, rstd[u], largest, &scale);
-          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = scale;
-          out[c] = (unsigned char)encode2(a[e] * f, 0.f, p.code);
+          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = code_scale(m, rstd[u], largest);
+          const float v = e & 1 ? a[e / 2].get().y : a[e / 2].get().x;
+          out[c] = (unsigned char)encode1(v * code_factor(m, rstd[u], largest), p.code);
         }
       }
     }
@@ -328,14 +396,20 @@ struct NormGradParams {
   int cols, weight_f32;
 };
 
+// How much of h the gradient loses: with d = sum(dy w h), rstd n mean(dy w n) = h * rstd^3 d / cols, one factor at a time.
+__device__ __forceinline__ float along(float d, float rstd, int cols) { return d * rstd / (float)cols * rstd * rstd; }
+
 // Writes a block's sums of the weight gradient to its row of the partial sums; teams that
 // share the block are added in shared memory, in their order.
 template <typename T, int TEAM, int NV, bool VEC>
-__device__ __forceinline__ void store_partial(const NormGradParams& p, const float* acc, float* shared) {
+__device__ __forceinline__ void store_partial(const NormGradParams& p, const Pair* sums, float* shared) {
   constexpr int E = Elem<T>::E;
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   float* mine = p.partial + (long long)blockIdx.x * cols;
   float* to = TEAM ? shared + threadIdx.y * cols : mine;
+  float acc[NV * E];
+#pragma unroll
+  for (int i = 0; i < NV * E; ++i) acc[i] = i & 1 ? sums[i / 2].get().y : sums[i / 2].get().x;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = column<T, VEC>(i, 0, me, team);
@@ -372,9 +446,9 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
     if (me < 64) slot[me >> 5][me & 31] = 0.f;
     __syncthreads();
   }
-  float acc[NV * E];
+  Pair acc[NV * E / 2];
 #pragma unroll
-  for (int i = 0; i < NV * E; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NV * E / 2; ++i) acc[i] = twice(0.f);
   int turn = 0;
   for (long long base = (long long)blockIdx.x * blockDim.y * RU; base < p.rows;
        base += (long long)gridDim.x * blockDim.y * RU, turn ^= 1) {
@@ -397,42 +471,44 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float w[E];
-      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      Pair w[E / 2];
+      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
-        float a[E], b[E];
-        Elem<T>::unpack(g[u][i], a);
-        Elem<T>::unpack(h[u][i], b);
+        Pair a[E / 2], b[E / 2], d(0.f, 0.f);
+        unpack2<T>(g[u][i], a);
+        unpack2<T>(h[u][i], b);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float n = b[e] * rstd[u];
-          dot[u] = fmaf(a[e] * w[e], n, dot[u]);
-          acc[i * E + e] = fmaf(a[e], n, acc[i * E + e]);
+        for (int e = 0; e < E / 2; ++e) {
+          d = fma2(a[e] * w[e], b[e], d);
+          acc[i * E / 2 + e] = fma2(a[e], b[e] * twice(rstd[u]), acc[i * E / 2 + e]);
         }
+        dot[u] += d.get().x + d.get().y;
       }
     }
     team_reduce<Sum, TEAM>(dot, slot[turn]);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float w[E];
-      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      Pair w[E / 2];
+      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         const long long row = base + u * blockDim.y + threadIdx.y;
-        const float mean = dot[u] / (float)cols;
-        float a[E], b[E], c[E];
-        Elem<T>::unpack(g[u][i], a);
-        Elem<T>::unpack(h[u][i], b);
-        Elem<T>::unpack(r[u][i], c);
+        const Pair back = twice(-along(dot[u], rstd[u], cols)), scale = twice(rstd[u]);
+        Pair a[E / 2], b[E / 2], c[E / 2];
+        unpack2<T>(g[u][i], a);
+        unpack2<T>(h[u][i], b);
+        unpack2<T>(r[u][i], c);
 #pragma unroll
-        for (int e = 0; e < E; ++e) a[e] = rstd[u] * (a[e] * w[e] - b[e] * rstd[u] * mean) + c[e];
-        if (row < p.rows) store_part<T, VEC>(p.grad_x + row * cols * S, i, me, team, cols, Elem<T>::pack(a));
+        for (int e = 0; e < E / 2; ++e) a[e] = fma2(a[e] * w[e], scale, fma2(back, b[e], c[e]));
+        if (row < p.rows) store_part<T, VEC>(p.grad_x + row * cols * S, i, me, team, cols, pack2<T>(a));
       }
     }
   }
   if (p.partial) store_partial<T, TEAM, NV, VEC>(p, acc, shared);
 }
+
+__host__ __device__ constexpr int ring_stages(int vectors) { return vectors == 4 ? 2 : 4; }
 
 __device__ __forceinline__ void copy_async(uint4* to, const char* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
@@ -443,8 +519,8 @@ __device__ __forceinline__ void copy_async(uint4* to, const char* from) {
 // thread's copy; the sums of the weight gradient (and up to 16 weights a thread) stay in
 // registers for all of the block's rows.
 template <typename T, int TEAM, int NV, bool RESIDUAL>
-__global__ void __launch_bounds__(TEAM ? kThreads : 512) rms_norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
-  constexpr int E = Elem<T>::E, STAGES = NV == 4 ? 2 : 4, TENSORS = RESIDUAL ? 3 : 2;
+__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
+  constexpr int E = Elem<T>::E, STAGES = ring_stages(NV), TENSORS = RESIDUAL ? 3 : 2;
   constexpr long long S = sizeof(T);
   extern __shared__ __align__(16) uint4 ring[];  // [STAGES][TENSORS][NV][threads]
   __shared__ __align__(16) float slot[2][32];
@@ -472,16 +548,18 @@ __global__ void __launch_bounds__(TEAM ? kThreads : 512) rms_norm_grad_ring_kern
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) fetch(s, row + s * step);
   constexpr bool KEEP = NV * E <= 16;  // the weights in registers; more of them are read again for each row
-  float w[KEEP ? NV * E : E], acc[NV * E];
+  Pair w[(KEEP ? NV * E : E) / 2], acc[NV * E / 2];
   if (KEEP) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, w + i * E);
+    for (int i = 0; i < NV; ++i) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, w + i * E / 2);
   }
 #pragma unroll
-  for (int i = 0; i < NV * E; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NV * E / 2; ++i) acc[i] = twice(0.f);
   int stage = 0, turn = 0;
+  float next_rstd = row < p.rows ? p.rstd[row] : 0.f;
   for (; row < p.rows; row += step, turn ^= 1) {
-    const float rstd = p.rstd[row];
+    const float rstd = next_rstd;
+    if (row + step < p.rows) next_rstd = p.rstd[row + step];
     // The stage that the previous row has left.
     fetch(stage == 0 ? STAGES - 1 : stage - 1, row + (STAGES - 1) * step);
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
@@ -495,35 +573,31 @@ __global__ void __launch_bounds__(TEAM ? kThreads : 512) rms_norm_grad_ring_kern
         g[i] = from[(0 * NV + i) * threads];
         h[i] = from[(1 * NV + i) * threads];
       }
-      float a[E], b[E], *wi = w + (KEEP ? i * E : 0);
-      if (!KEEP) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
-      Elem<T>::unpack(g[i], a);
-      Elem<T>::unpack(h[i], b);
+      Pair a[E / 2], b[E / 2], *wi = w + (KEEP ? i * E / 2 : 0), d(0.f, 0.f);
+      if (!KEEP) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
+      unpack2<T>(g[i], a);
+      unpack2<T>(h[i], b);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float n = b[e] * rstd;
-        dot[0] = fmaf(a[e] * wi[e], n, dot[0]);
-        acc[i * E + e] = fmaf(a[e], n, acc[i * E + e]);
+      for (int e = 0; e < E / 2; ++e) {
+        d = fma2(a[e] * wi[e], b[e], d);
+        acc[i * E / 2 + e] = fma2(a[e], b[e] * twice(rstd), acc[i * E / 2 + e]);
       }
+      dot[0] += d.get().x + d.get().y;
     }
     team_reduce<Sum, TEAM>(dot, slot[turn]);
-    const float mean = dot[0] / (float)cols;
+    const Pair back = twice(-along(dot[0], rstd, cols)), scale = twice(rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = column<T, true>(i, 0, me, team);
       if (c >= cols) continue;
-      float a[E], b[E], *wi = w + (KEEP ? i * E : 0);
-      if (!KEEP) load_weight<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
-      Elem<T>::unpack(g[i], a);
-      Elem<T>::unpack(h[i], b);
+      Pair a[E / 2], b[E / 2], f[E / 2], *wi = w + (KEEP ? i * E / 2 : 0);
+      if (!KEEP) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
+      unpack2<T>(g[i], a);
+      unpack2<T>(h[i], b);
+      if (RESIDUAL) unpack2<T>(from[(2 * NV + i) * threads], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) a[e] = rstd * (a[e] * wi[e] - b[e] * rstd * mean);
-      if (RESIDUAL) {
-        Elem<T>::unpack(from[(2 * NV + i) * threads], b);
-#pragma unroll
-        for (int e = 0; e < E; ++e) a[e] += b[e];
-      }
-      *reinterpret_cast<uint4*>(p.grad_x + (row * cols + c) * S) = Elem<T>::pack(a);
+      for (int e = 0; e < E / 2; ++e) a[e] = fma2(a[e] * wi[e], scale, RESIDUAL ? fma2(back, b[e], f[e]) : back * b[e]);
+      *reinterpret_cast<uint4*>(p.grad_x + (row * cols + c) * S) = pack2<T>(a);
     }
     stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
@@ -539,8 +613,10 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* par
   __shared__ float s[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int i = threadIdx.y; i < parts; i += 32) v += partial[(long long)i * cols + c];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   v = s[threadIdx.x][threadIdx.y];
@@ -566,6 +642,15 @@ RowShape row_shape(int cols, int elems, bool vec) {
   }
   const int vectors = parts <= 512 ? 2 : parts <= 4096 ? 4 : 8;
   return {(int)ceil_div(ceil_div(parts, vectors), 32) * 32, vectors, 1};
+}
+
+// The backward pass keeps the weights and their gradient in registers: two parts a thread wherever that will do, and so
+// a block already for rows of more than 64 parts (1024 columns of bfloat16, 32768 rows: 55.7 us with four parts in a
+// warp, which reads the weights again for each row).
+RowShape grad_shape(int cols, int elems, bool vec) {
+  const int parts = (int)ceil_div(cols, elems);
+  if (!vec || parts <= 64 || parts > 128) return row_shape(cols, elems, vec);
+  return {64, 2, 1};
 }
 
 template <typename T, bool VEC, bool CODES>
@@ -612,11 +697,9 @@ const void* norm_grad_kernel_of(const RowShape& s) {
 }
 template <typename T, bool RESIDUAL>
 const void* norm_grad_ring_of(const RowShape& s) {
-  if (s.lanes() == 32) {
-    if (s.vectors == 1) return (const void*)rms_norm_grad_ring_kernel<T, 32, 1, RESIDUAL>;
-    if (s.vectors == 2) return (const void*)rms_norm_grad_ring_kernel<T, 32, 2, RESIDUAL>;
-    return (const void*)rms_norm_grad_ring_kernel<T, 32, 4, RESIDUAL>;
-  }
+  if (s.lanes() == 32)
+    return s.vectors == 1 ? (const void*)rms_norm_grad_ring_kernel<T, 32, 1, RESIDUAL>
+                          : (const void*)rms_norm_grad_ring_kernel<T, 32, 2, RESIDUAL>;
   if (s.vectors == 2) return (const void*)rms_norm_grad_ring_kernel<T, 0, 2, RESIDUAL>;
   return (const void*)rms_norm_grad_ring_kernel<T, 0, 4, RESIDUAL>;
 }
@@ -628,14 +711,16 @@ const void* norm_grad_kernel(const RowShape& s, bool vec, bool residual) {
 
 // Shared memory of a backward block.
 size_t grad_shared(const RowShape& s, bool vec, bool residual, int64_t cols) {
-  if (ring_takes(s, vec)) return (size_t)(s.vectors == 4 ? 2 : 4) * (residual ? 3 : 2) * s.vectors * s.team * s.teams * 16;
+  if (ring_takes(s, vec)) return (size_t)ring_stages(s.vectors) * (residual ? 3 : 2) * s.vectors * s.team * s.teams * 16;
   return s.teams > 1 ? (size_t)s.teams * cols * sizeof(float) : 0;
 }
 
-// Blocks of the backward pass: as many as fit an SM, four at most, and no more than there are rows for.
+// Blocks of the backward pass: as many as fit an SM by their shared memory and at 128 registers a thread, eight at most,
+// and no more than there are rows for.
 int grad_blocks(const RowShape& s, size_t shared, int64_t rows) {
-  const int64_t fit = shared ? (int64_t)(220 << 10) / (int64_t)shared : 4;
-  const int64_t most = kSMs * (fit < 1 ? 1 : fit > 4 ? 4 : fit), sets = ceil_div(rows, s.teams);
+  const int64_t by_shared = shared ? (int64_t)(220 << 10) / (int64_t)shared : 8, by_threads = 512 / (s.team * s.teams);
+  const int64_t fit = by_shared < by_threads ? by_shared : by_threads;
+  const int64_t most = kSMs * (fit < 1 ? 1 : fit > 8 ? 8 : fit), sets = ceil_div(rows, s.teams);
   return (int)(sets < most ? sets : most);
 }
 
@@ -742,7 +827,7 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
                    hidden_stride % elems == 0 && aligned(grad_x, 16) && (!weight || aligned(weight, 16)) &&
                    (!grad_hidden || (aligned(grad_hidden, 16) && grad_hidden_stride % elems == 0)) &&
                    aligned(workspace, 16);
-  const RowShape s = row_shape((int)cols, elems, vec);
+  const RowShape s = grad_shape((int)cols, elems, vec);
   const size_t smem = grad_shared(s, vec, grad_hidden != nullptr, cols);
   const int parts = grad_blocks(s, smem, rows);
   if (grad_weight && workspace_bytes < (int64_t)parts * cols * (int64_t)sizeof(float))
