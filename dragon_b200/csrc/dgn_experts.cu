@@ -31,14 +31,25 @@ struct RouteParams {
   float* weights;
   long long tokens, stride;
   int experts, k, sigmoid, groups, keep, best, renormalize;
+  int bits;        // of an expert's number
+  unsigned magic;  // e * magic >> 20 is expert e's group
   float scale;
 };
 
 // Keys as whole numbers that sort like the values: 0 is "not to be chosen", NaN comes first.
 __device__ __forceinline__ u64 order_of(double v) {
   if (isnan(v)) return ~0ull;
+  if (isinf(v) && v < 0) return 0;
   const u64 bits = (u64)__double_as_longlong(v + 0.0);  // -0 becomes 0
   return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+// The same for float32, and back.
+__device__ __forceinline__ unsigned order_of(float v) {
+  const unsigned bits = __float_as_uint(v + 0.f);
+  return bits >> 31 ? ~bits : bits | 1u << 31;
+}
+__device__ __forceinline__ float value_of(unsigned order) {
+  return __uint_as_float(order >> 31 ? order ^ 1u << 31 : ~order);
 }
 
 // Largest key of a warp and the lowest index that has it.
@@ -54,72 +65,45 @@ __device__ __forceinline__ void first_largest(u64* key, int* index) {
   }
 }
 
-// One warp for a token, N experts for a lane: lane l holds experts l, l + 32, ...
-template <typename T, int N>
-__global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long token = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (token >= p.tokens) return;
-  int* indices = p.indices + token * p.k;
-  float* weights = p.weights + token * p.k;
-  if (p.mask && !p.mask[token]) {
-    if (lane < p.k) {
-      indices[lane] = -1;
-      weights[lane] = 0.f;
-    }
-    return;
-  }
+// One token's choice in 64 bits by a whole warp, its keys in shared memory.  Taken by the
+// tokens whose choice hangs on values that float32 does not tell apart, and by those that
+// hold a NaN or an infinity: a few in a thousand, so it is made small, not fast.
+template <typename T>
+__device__ __noinline__ void route_exact(const RouteParams& p, long long token, double* key) {
+  const int lane = threadIdx.x & 31, experts = p.experts;
   const T* row = reinterpret_cast<const T*>(p.logits) + token * p.stride;
-  double score[N];
-  u64 key[N];
-  double top = -INFINITY;
+  double top = -INFINITY, sum = 0.0;
+  for (int e = lane; e < experts; e += 32) top = fmax(top, (double)widen(row[e]));
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    score[i] = e < p.experts ? (double)widen(row[e]) : -INFINITY;
-    key[i] = isinf(score[i]) && score[i] < 0 ? 0 : order_of(score[i]);
-    top = fmax(top, score[i]);
-  }
-  if (p.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) score[i] = 1.0 / (1.0 + exp(-score[i]));
-  } else {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      score[i] = key[i] ? exp(score[i] - top) : 0.0;
-      sum += score[i];
-    }
+  for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
+  const auto raised = [&](double l) { return isinf(l) && l < 0 ? 0.0 : exp(l - top); };
+  if (!p.sigmoid) {
+    for (int e = lane; e < experts; e += 32) sum += raised(widen(row[e]));
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-#pragma unroll
-    for (int i = 0; i < N; ++i) score[i] = key[i] ? score[i] / sum : 0.0;
   }
-  if (p.bias) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = i * 32 + lane;
-      if (!key[i]) continue;
-      const double v = score[i] + (double)p.bias[e];
-      key[i] = isinf(v) && v < 0 ? 0 : order_of(v);
-    }
+  const auto score = [&](int e) {
+    const double l = widen(row[e]);
+    return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : raised(l) / sum;
+  };
+  __syncwarp();
+  for (int e = lane; e < experts; e += 32) {
+    const double l = widen(row[e]);
+    key[e] = p.bias && !(isinf(l) && l < 0) ? score(e) + (double)p.bias[e] : l;
   }
+  __syncwarp();
   if (p.groups > 1) {
-    const int width = p.experts / p.groups;
+    const int width = experts / p.groups;
     const bool by_key = p.bias || p.best == 1;  // otherwise the score is what is added up
-    u64 mine = 0;  // lane g: the value of group g
+    u64 mine = 0;                               // lane g: the value of group g
     for (int g = 0; g < p.groups; ++g) {
       u64 a = 0, b = 0;  // the two largest, by order
       int ia = kMaxExperts, ib = kMaxExperts;
       double va = 0.0, vb = 0.0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int e = i * 32 + lane;
-        if (e / width != g || !key[i]) continue;
-        const double v = p.bias ? score[i] + (double)p.bias[e] : score[i];
-        const u64 o = by_key ? key[i] : order_of(v);
+      for (int e = g * width + lane; e < (g + 1) * width; e += 32) {
+        if (!order_of(key[e])) continue;
+        const double v = by_key ? key[e] : score(e);
+        const u64 o = order_of(v);
         if (o > a) {
           b = a; ib = ia; vb = va;
           a = o; ia = e; va = v;
@@ -153,46 +137,274 @@ __global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ Rout
       kept |= 1u << g;
       if (lane == g) mine = 0;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (!(kept >> min((i * 32 + lane) / width, 31) & 1)) key[i] = 0;
+    __syncwarp();
+    for (int e = lane; e < experts; e += 32)
+      if (!(kept >> (e / width) & 1)) key[e] = -INFINITY;
+    __syncwarp();
   }
   int index = -1;
-  float s = 0.f;
   for (int n = 0; n < p.k; ++n) {
     u64 best = 0;
     int at = kMaxExperts;
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = i * 32 + lane;
-        v = (float)score[i];
+    for (int e = lane; e < experts; e += 32) {
+      const u64 o = order_of(key[e]);
+      if (o > best) {
+        best = o;
+        at = e;
       }
-    int e = at;
-    first_largest(&best, &e);
-    if (!best) break;
-    const float chosen = __shfl_sync(kFull, v, e & 31);
-    if (lane == n) {
-      index = e;
-      s = chosen;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 32 + lane == e) key[i] = 0;
+    first_largest(&best, &at);
+    if (!best) break;
+    if (lane == n) index = at;
+    if (lane == (at & 31)) key[at] = -INFINITY;
+    __syncwarp();
   }
+  const float s = index < 0 ? 0.f : (float)score(index);
   float w = s;
   if (p.renormalize) {
-    float sum = s;
+    float total = s;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-    w = s / (sum + kTiny);
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(kFull, total, d);
+    w = s / (total + kTiny);
   }
   if (lane < p.k) {
-    indices[lane] = index;
-    weights[lane] = index < 0 ? 0.f : w * p.scale;
+    p.indices[token * p.k + lane] = index;
+    p.weights[token * p.k + lane] = index < 0 ? 0.f : w * p.scale;
   }
+}
+
+// exp(x) to about 2^-22 of its largest value in a row of differences to the maximum.
+__device__ __forceinline__ float quick_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float quick_sigmoid(float x) { return __fdividef(1.f, 1.f + quick_exp(-x)); }
+
+// N logits of a row for each of L lanes in float32, -inf behind the last.  VEC: 16 bytes
+// at a time, lane l has vectors l, l + L, ...; otherwise elements l, l + L, ...
+template <typename T, int L, bool VEC>
+__device__ __forceinline__ int expert_of(int i, int lane) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+  return (i / V * L + lane) * V + i % V;
+}
+template <typename T, int L, int N, bool VEC>
+__device__ __forceinline__ void load_logits(const T* row, bool live, int experts, int lane, float* x) {
+  if constexpr (VEC) {
+    constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      if (live && e < experts) {
+        Elem<T>::unpack(*reinterpret_cast<const uint4*>(row + e), x + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i + j] = -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      x[i] = live && e < experts ? widen(row[e]) : -INFINITY;
+    }
+  }
+}
+
+template <int L> __device__ __forceinline__ float team_sum(float v) {
+#pragma unroll
+  for (int d = L / 2; d; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  return v;
+}
+template <int L> __device__ __forceinline__ float team_max(float v) {
+#pragma unroll
+  for (int d = L / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, d));
+  return v;
+}
+template <int L> __device__ __forceinline__ unsigned team_max(unsigned v) {
+#pragma unroll
+  for (int d = L / 2; d; d >>= 1) v = max(v, __shfl_xor_sync(kFull, v, d));
+  return v;
+}
+
+constexpr int kRouteThreads = 128;
+
+// Shared memory of one warp: its teams' keys by group, or the keys of route_exact; then each team's winners and group values.
+__host__ __device__ inline int route_values(int experts, int groups, int teams) {
+  const int grouped = groups > 1 ? teams * (experts + groups) * 4 : 0;
+  return (max(grouped, experts * 8) + 15) / 16 * 16;
+}
+__host__ __device__ inline int route_shared(int experts, int groups, int teams) {
+  return route_values(experts, groups, teams) + teams * (kMaxChoices + 1 + kMaxGroups + 3) * 4;
+}
+
+// L lanes for a token, N experts for a lane; experts <= 1 << bits <= L * N.
+//
+// What bounds it is the number of instructions, not the bytes: 5 of each logit's bytes take
+// a fraction of the time of k passes over it.  A key in float32 and its expert's number are
+// one 31-bit word: the key's order without its lowest bits, which hold the number, the lowest
+// the largest.  So the words differ, one maximum finds value and place at once, and the
+// next largest is the largest of word - last, wrapped around, without anything being marked.
+// The choice stands if float32 tells each of the k + 1 first words from the next (by the
+// gap between what their upper bits leave open, less the rounding of the scores where there
+// is a bias); otherwise route_exact makes it again.  16-bit logits lose nothing with the lowest bits.
+template <typename T, int L, int N, bool VEC>
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteParams p) {
+  constexpr int TEAMS = 32 / L;
+  constexpr unsigned kWrap = 1u << 31;
+  extern __shared__ __align__(16) char shared[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x % L, team = (threadIdx.x & 31) / L, experts = p.experts;
+  char* mine = shared + warp * route_shared(experts, p.groups, TEAMS);
+  unsigned* win = reinterpret_cast<unsigned*>(mine + route_values(experts, p.groups, TEAMS)) +
+                  team * (kMaxChoices + 1 + kMaxGroups + 3);
+  float* group_value = reinterpret_cast<float*>(win + kMaxChoices + 1);
+  const long long token = ((long long)blockIdx.x * (kRouteThreads / 32) + warp) * TEAMS + team;
+  const bool live = token < p.tokens && !(p.mask && !p.mask[token]);
+  const T* row = reinterpret_cast<const T*>(p.logits) + (live ? token : 0) * p.stride;
+  const unsigned low = (1u << p.bits) - 1;
+
+  float x[N];
+  load_logits<T, L, N, VEC>(row, live, experts, lane, x);
+  bool odd = false;  // what float32 does not decide
+#pragma unroll
+  for (int i = 0; i < N; ++i) odd |= !(x[i] < INFINITY);
+  // Scores of all experts are needed with a bias, and their sum unless it cancels in the weights.
+  const bool plain = !p.bias && p.groups == 1;
+  float top = 0.f, inv = 1.f, largest_score = 1.f;
+  if (!p.sigmoid && !(plain && p.renormalize)) {
+    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+    top = team_max<L>(top);
+    if (top == -INFINITY) top = 0.f;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i & 3] += quick_exp(x[i] - top);
+    inv = largest_score = 1.f / team_sum<L>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  }
+  const auto quick_score = [&](float l) { return p.sigmoid ? quick_sigmoid(l) : quick_exp(l - top) * inv; };
+  // Twice what a score may be off by: 2^-22 of the largest for its exponential, 15 additions and a quotient at 2^-24.
+  const float slack = largest_score * 0x1p-18f;
+
+  unsigned kept = ~0u;
+  const int width = experts / p.groups;
+  if (p.groups > 1) {
+    float* values = reinterpret_cast<float*>(mine) + team * (experts + p.groups);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      if (e >= experts) continue;
+      const float v = x[i] == -INFINITY ? x[i]
+                      : p.bias          ? quick_score(x[i]) + p.bias[e]
+                      : p.best == 2     ? quick_score(x[i])
+                                        : x[i];
+      values[e + (e * p.magic >> 20)] = v;  // a word between the groups keeps them in different banks
+    }
+    __syncwarp();
+    for (int g = lane; g < p.groups; g += L) {
+      float a = -INFINITY, b = -INFINITY;
+      for (int i = 0; i < width; ++i) {
+        const float v = values[g * (width + 1) + i];
+        b = fmaxf(b, fminf(a, v));
+        a = fmaxf(a, v);
+      }
+      group_value[g] = p.best == 2 && b > -INFINITY ? a + b : a;
+    }
+    __syncwarp();
+    unsigned bits = 0;
+    float worst = INFINITY, next = -INFINITY;  // the values on either side of the border
+    for (int g = lane; g < p.groups; g += L) {
+      const float v = group_value[g];
+      int rank = 0;
+      for (int o = 0; o < p.groups; ++o) rank += group_value[o] > v || (group_value[o] == v && o < g);
+      if (rank < p.keep) {
+        bits |= 1u << g;
+        worst = fminf(worst, v);
+      } else {
+        next = fmaxf(next, v);
+      }
+    }
+#pragma unroll
+    for (int d = L / 2; d; d >>= 1) {
+      bits |= __shfl_xor_sync(kFull, bits, d);
+      worst = fminf(worst, __shfl_xor_sync(kFull, worst, d));
+      next = fmaxf(next, __shfl_xor_sync(kFull, next, d));
+    }
+    kept = bits;
+    // Logits alone are compared as they are; sums and scores have to be further apart than they may be off.
+    if ((p.bias || p.best == 2) && p.keep < p.groups && next > -INFINITY)
+      odd |= !(worst - next > 2.f * slack + 0x1p-20f * (fabsf(worst) + fabsf(next)));
+  }
+
+  unsigned word[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = expert_of<T, L, VEC>(i, lane);
+    float v = x[i];
+    if (p.bias && e < experts && v > -INFINITY) {
+      v = quick_score(v) + p.bias[e];
+      odd |= !(v < INFINITY);
+    }
+    word[i] = v > -INFINITY && (kept >> (e * p.magic >> 20 & 31) & 1) ? (order_of(v) >> 1 & ~low) | (low - e) : 0;
+  }
+  unsigned last = kWrap;
+  const int wanted = p.k + (sizeof(T) == 2 && !p.bias ? 0 : 1);
+  for (int j = 0; j < wanted; ++j) {
+    unsigned best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = max(best, word[i] - last);
+    best = best >= kWrap ? best + last : 0;
+    last = team_max<L>(best);
+    if (lane == j % L) win[j] = last;
+    if (last == 0) last = 1;  // nothing is left: only zeros stay below
+  }
+  __syncwarp();
+
+  // Choice j belongs to lane j % L.
+  float score[kMaxChoices / L];
+  int index[kMaxChoices / L];
+  const float first = plain && p.renormalize && !p.sigmoid && win[0] ? widen(row[low - (win[0] & low)]) : top;
+  float total = 0.f;
+#pragma unroll
+  for (int q = 0; q < kMaxChoices / L; ++q) {
+    const int j = q * L + lane;
+    index[q] = -1;
+    score[q] = 0.f;
+    if (j >= p.k || !win[j]) continue;
+    index[q] = low - (win[j] & low);
+    const float l = widen(row[index[q]]);
+    score[q] = p.sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - first) * inv;
+    total += score[q];
+    const unsigned after = j + 1 < wanted ? win[j + 1] : 0;
+    if (!after) continue;
+    if (!p.bias) {
+      odd |= sizeof(T) == 4 && (win[j] & ~low) == (after & ~low);
+    } else {
+      const float floor = value_of((win[j] & ~low) << 1), ceiling = value_of(((after | low) + 1) << 1);
+      if (!(floor - ceiling > slack + 0x1p-21f * fabsf(floor))) {
+        // Two experts with the same logit and bias are in order; behind the last choice there may be more to see.
+        const int other = low - (after & low);
+        odd |= j + 1 == p.k || widen(row[other]) != l || p.bias[other] != p.bias[index[q]];
+      }
+    }
+  }
+  total = p.renormalize ? team_sum<L>(total) + kTiny : 1.f;
+  const unsigned again = __ballot_sync(kFull, odd && live);
+  const unsigned ours = L == 32 ? ~0u : ((1u << (L & 31)) - 1) << (team * L);
+  if (token < p.tokens && !(again & ours)) {
+#pragma unroll
+    for (int q = 0; q < kMaxChoices / L; ++q) {
+      const int j = q * L + lane;
+      if (j >= p.k) continue;
+      p.indices[token * p.k + j] = index[q];
+      p.weights[token * p.k + j] = index[q] < 0 ? 0.f : (p.renormalize ? score[q] / total : score[q]) * p.scale;
+    }
+  }
+  __syncwarp();
+#pragma unroll 1
+  for (int t = 0; t < TEAMS; ++t)
+    if (again & (L == 32 ? ~0u : ((1u << (L & 31)) - 1) << (t * L)))
+      route_exact<T>(p, token - team + t, reinterpret_cast<double*>(mine));
 }
 
 struct RouteGradParams {
@@ -205,88 +417,109 @@ struct RouteGradParams {
   float scale;
 };
 
-template <typename T, int N>
-__global__ void __launch_bounds__(128) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long token = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (token >= p.tokens) return;
-  const T* row = reinterpret_cast<const T*>(p.logits) + token * p.stride;
-  T* grad = reinterpret_cast<T*>(p.grad) + token * p.experts;
-  float score[N];
-  float top = -INFINITY;
+// The gradient of the scores is zero but for the k choices: those are put into a row of
+// shared memory, and each lane picks up its own experts'.
+template <typename T, int L, int N, bool VEC>
+__global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
+  constexpr int Q = kMaxChoices / L, V = VEC ? 16 / (int)sizeof(T) : 1;
+  __shared__ float direct[kRouteThreads / L][N * L];
+  __shared__ int chosen[kRouteThreads / L][kMaxChoices];
+  __shared__ float slope[kRouteThreads / L][kMaxChoices];
+  const int lane = threadIdx.x % L, team = threadIdx.x / L, experts = p.experts;
+  const long long token = (long long)blockIdx.x * (kRouteThreads / L) + team;
+  const bool live = token < p.tokens;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (live ? token : 0) * p.stride;
+  float x[N];
+  load_logits<T, L, N, VEC>(row, live, experts, lane, x);
+  int index[Q];
+  float ds[Q], logit[Q];
+  bool any = false;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    score[i] = e < p.experts ? widen(row[e]) : -INFINITY;
-    top = fmaxf(top, score[i]);
+  for (int q = 0; q < Q; ++q) {
+    const int j = q * L + lane;
+    index[q] = live && j < p.k ? p.indices[token * p.k + j] : -1;
+    if (index[q] < 0 || index[q] >= experts) index[q] = -1;
+    any |= index[q] >= 0;
+    ds[q] = index[q] < 0 ? 0.f : p.scale * p.grad_weights[token * p.k + j];
+    logit[q] = index[q] < 0 ? -INFINITY : widen(row[index[q]]);
   }
-  // The chosen experts: lane j < k holds choice j.
-  int index = lane < p.k ? p.indices[token * p.k + lane] : -1;
-  if (index >= p.experts) index = -1;
-  float ds = index < 0 ? 0.f : p.scale * p.grad_weights[token * p.k + lane];
-  if (index < 0) index = -1;
-  if (!__ballot_sync(kFull, index >= 0)) {  // a padded token: whatever its logits hold, no gradient
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 32 + lane < p.experts) grad[i * 32 + lane] = T(0.f);
-    return;
-  }
-  const float logit = index < 0 ? -INFINITY : widen(row[index]);
-  float mine;
-  if (p.sigmoid) {
+  for (int i = 0; i < N; ++i) direct[team][i * L + lane] = 0.f;
+  float top = 0.f, inv = 1.f;
+  if (!p.sigmoid) {
+    top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {  // s (1 - s) without the cancellation near 1
-      const float t = expf(-fabsf(score[i]));
-      score[i] = t / ((1.f + t) * (1.f + t));
-    }
-    mine = index < 0 ? 0.f : 1.f / (1.f + expf(-logit));
-  } else {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-    float sum = 0.f;
+    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
+    top = team_max<L>(top);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      score[i] = score[i] == -INFINITY ? 0.f : expf(score[i] - top);
-      sum += score[i];
+      x[i] = x[i] == -INFINITY ? 0.f : quick_exp(x[i] - top);  // a NaN stays one
+      sum[i & 3] += x[i];
     }
+    const float all = team_sum<L>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    inv = all == 0.f ? 0.f : 1.f / all;
+  }
+  float mine[Q], total = 0.f, dot = 0.f;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-#pragma unroll
-    for (int i = 0; i < N; ++i) score[i] = score[i] == 0.f ? 0.f : score[i] / sum;
-    mine = index < 0 || logit == -INFINITY ? 0.f : expf(logit - top) / sum;
+  for (int q = 0; q < Q; ++q) {
+    mine[q] = logit[q] == -INFINITY ? 0.f : p.sigmoid ? 1.f / (1.f + expf(-logit[q])) : expf(logit[q] - top) * inv;
+    total += mine[q];
+    dot += ds[q] * mine[q];
   }
   if (p.renormalize) {
-    float total = mine, dot = ds * mine;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-      total += __shfl_xor_sync(kFull, total, d);
-      dot += __shfl_xor_sync(kFull, dot, d);
-    }
-    total += kTiny;
-    ds = index < 0 ? 0.f : (ds - dot / total) / total;
-  }
-  float dot = ds * mine;
-  if (p.sigmoid) {
+    total = team_sum<L>(total) + kTiny;
+    const float along = team_sum<L>(dot) / total;
     dot = 0.f;
-  } else {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
+    for (int q = 0; q < Q; ++q) {
+      ds[q] = index[q] < 0 ? 0.f : (ds[q] - along) / total;
+      dot += ds[q] * mine[q];
+    }
   }
-  float direct[N];
+  dot = p.sigmoid ? 0.f : team_sum<L>(dot);
 #pragma unroll
-  for (int i = 0; i < N; ++i) direct[i] = 0.f;
-  for (int j = 0; j < p.k; ++j) {
-    const int e = __shfl_sync(kFull, index, j);
-    const float d = __shfl_sync(kFull, ds, j);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 32 + lane == e) direct[i] += d;
+  for (int q = 0; q < Q; ++q) {
+    const int j = q * L + lane;
+    if (j < p.k) {
+      chosen[team][j] = index[q];
+      slope[team][j] = ds[q];
+    }
   }
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    const float s = score[i];
-    if (e < p.experts) grad[e] = T(p.sigmoid ? direct[i] * s : s * (direct[i] - dot));
+  for (int q = 0; q < Q; ++q) {
+    if (index[q] < 0) continue;
+    float all = 0.f;  // an expert that stands twice counts twice, in the order of the choices
+    for (int j = 0; j < p.k; ++j)
+      if (chosen[team][j] == index[q]) all += slope[team][j];
+    direct[team][index[q]] = all;
+  }
+  const unsigned ballot = __ballot_sync(kFull, any);
+  const bool empty = !(ballot & (L == 32 ? ~0u : ((1u << (L & 31)) - 1) << ((threadIdx.x & 31) / L * L)));
+  if (!live) return;
+  T* grad = reinterpret_cast<T*>(p.grad) + token * experts;
+#pragma unroll
+  for (int i = 0; i < N; i += V) {
+    const int e = expert_of<T, L, VEC>(i, lane);
+    if (e >= experts) break;
+    float g[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = direct[team][e + j];
+      if (p.sigmoid) {  // s (1 - s) without the cancellation near 1
+        const float t = quick_exp(-fabsf(x[i + j])), u = __fdividef(1.f, 1.f + t);
+        g[j] = d * t * u * u;
+      } else {
+        g[j] = x[i + j] * inv * (d - dot);
+      }
+      if (empty) g[j] = 0.f;  // a padded token: whatever its logits hold, no gradient
+    }
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(grad + e) = Elem<T>::pack(g);
+    } else {
+      grad[e] = T(g[0]);
+    }
   }
 }
 
@@ -573,21 +806,25 @@ __global__ void __launch_bounds__(1024) update_bias_kernel(const float* bias, co
 
 // ---- kernel choice -----------------------------------------------------------------------------
 
-template <typename T>
+// Lanes for a token: eight where 16 experts a lane suffice, so that a warp works on four tokens at once, and more as
+// the experts become more.
+int route_lanes(int experts) { return experts <= 128 ? 8 : experts <= 256 ? 16 : 32; }
+
+template <typename T, bool VEC>
 const void* route_fn(int experts) {
-  if (experts <= 64) return (const void*)route_kernel<T, 2>;
-  if (experts <= 128) return (const void*)route_kernel<T, 4>;
-  if (experts <= 256) return (const void*)route_kernel<T, 8>;
-  if (experts <= 512) return (const void*)route_kernel<T, 16>;
-  return (const void*)route_kernel<T, 32>;
+  if (experts <= 64) return (const void*)route_kernel<T, 8, 8, VEC>;
+  if (experts <= 128) return (const void*)route_kernel<T, 8, 16, VEC>;
+  if (experts <= 256) return (const void*)route_kernel<T, 16, 16, VEC>;
+  if (experts <= 512) return (const void*)route_kernel<T, 32, 16, VEC>;
+  return (const void*)route_kernel<T, 32, 32, VEC>;
 }
-template <typename T>
+template <typename T, bool VEC>
 const void* route_grad_fn(int experts) {
-  if (experts <= 64) return (const void*)route_grad_kernel<T, 2>;
-  if (experts <= 128) return (const void*)route_grad_kernel<T, 4>;
-  if (experts <= 256) return (const void*)route_grad_kernel<T, 8>;
-  if (experts <= 512) return (const void*)route_grad_kernel<T, 16>;
-  return (const void*)route_grad_kernel<T, 32>;
+  if (experts <= 64) return (const void*)route_grad_kernel<T, 8, 8, VEC>;
+  if (experts <= 128) return (const void*)route_grad_kernel<T, 8, 16, VEC>;
+  if (experts <= 256) return (const void*)route_grad_kernel<T, 16, 16, VEC>;
+  if (experts <= 512) return (const void*)route_grad_kernel<T, 32, 16, VEC>;
+  return (const void*)route_grad_kernel<T, 32, 32, VEC>;
 }
 template <typename T>
 const void* combine_fn(bool vec) {
@@ -660,12 +897,20 @@ extern "C" int dgn_route(const void* logits, int64_t stride, const float* bias, 
   p.best = best;
   p.renormalize = renormalize != 0;
   p.scale = scale;
-  const void* fn = dtype == DGN_F32   ? route_fn<float>(experts)
-                   : dtype == DGN_F16 ? route_fn<__half>(experts)
-                                      : route_fn<__nv_bfloat16>(experts);
+  p.bits = 1;
+  while (1 << p.bits < experts) ++p.bits;
+  p.magic = (unsigned)ceil_div(1 << 20, experts / groups);
+  const int elems = 16 / (int)dgn_dtype_size(dtype), teams = 32 / route_lanes(experts);
+  const bool vec = experts % elems == 0 && stride % elems == 0 && aligned(logits, 16);
+  const void* fn = dtype == DGN_F32   ? (vec ? route_fn<float, true>(experts) : route_fn<float, false>(experts))
+                   : dtype == DGN_F16 ? (vec ? route_fn<__half, true>(experts) : route_fn<__half, false>(experts))
+                   : vec              ? route_fn<__nv_bfloat16, true>(experts)
+                                      : route_fn<__nv_bfloat16, false>(experts);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)ceil_div(tokens, 4)), dim3(128), 0, stream, args);
+  const int warps = kRouteThreads / 32;
+  return launch(fn, dim3((unsigned)ceil_div(tokens, warps * teams)), dim3(kRouteThreads),
+                (size_t)warps * route_shared(experts, groups, teams), stream, args);
 }
 
 extern "C" int dgn_route_grad(const float* grad_weights, const void* logits, int64_t stride, const int32_t* indices,
@@ -690,12 +935,16 @@ extern "C" int dgn_route_grad(const float* grad_weights, const void* logits, int
   p.sigmoid = score == DGN_SCORE_SIGMOID;
   p.renormalize = renormalize != 0;
   p.scale = scale;
-  const void* fn = dtype == DGN_F32   ? route_grad_fn<float>(experts)
-                   : dtype == DGN_F16 ? route_grad_fn<__half>(experts)
-                                      : route_grad_fn<__nv_bfloat16>(experts);
+  const int elems = 16 / (int)es;
+  const bool vec = experts % elems == 0 && stride % elems == 0 && aligned(logits, 16) && aligned(grad_logits, 16);
+  const void* fn = dtype == DGN_F32   ? (vec ? route_grad_fn<float, true>(experts) : route_grad_fn<float, false>(experts))
+                   : dtype == DGN_F16 ? (vec ? route_grad_fn<__half, true>(experts) : route_grad_fn<__half, false>(experts))
+                   : vec              ? route_grad_fn<__nv_bfloat16, true>(experts)
+                                      : route_grad_fn<__nv_bfloat16, false>(experts);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)ceil_div(tokens, 4)), dim3(128), 0, stream, args);
+  return launch(fn, dim3((unsigned)ceil_div(tokens, kRouteThreads / route_lanes(experts))), dim3(kRouteThreads), 0, stream,
+                args);
 }
 
 extern "C" int64_t dgn_expert_plan_workspace(int64_t slots, int experts) {

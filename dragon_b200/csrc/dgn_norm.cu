@@ -39,7 +39,7 @@ struct NormParams {
   long long rows, x_stride, residual_stride, hidden_stride;  // strides in elements
   int cols, group_shift, groups;  // columns per scale as a power of two; scales per row
   int weight_f32, code;
-  float eps;
+  float eps, inv_cols, largest, inv_largest;  // the largest code
 };
 
 // Threads and columns.  A row belongs to a team of `team` threads; each of them holds NV
@@ -173,9 +173,10 @@ __device__ __forceinline__ void team_reduce(float (&v)[RU], float* slot) {
   if (TEAM) return;
   const int warps = blockDim.x >> 5;
   if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v[0];
+  if (threadIdx.x >= warps && threadIdx.x < 32) slot[threadIdx.x] = 0.f;
   __syncthreads();
   float all = 0.f;
-  for (int w = 0; w < warps; w += 4) {  // 32 slots, those of missing warps are zero
+  for (int w = 0; w < warps; w += 4) {
     const float4 f = *reinterpret_cast<const float4*>(slot + w);
     all = Op::of(all, Op::of(Op::of(f.x, f.y), Op::of(f.z, f.w)));
   }
@@ -205,20 +206,28 @@ __device__ __forceinline__ uint2 encode(const Pair* a, int code) {
   }
   return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
-__device__ __forceinline__ float largest_code(int code) {
-  return code == DGN_CODE_I8 ? 127.f : code == DGN_CODE_E4M3 ? 448.f : 57344.f;
-}
 
 // Codes of values h * w * rstd from u = h * w alone: with m the largest |u| of the group, code = rn(u * (L / m)) and
 // scale = m * rstd / L, so that rstd's rounding does not move a code.
+__device__ __forceinline__ float reciprocal(float m) {  // of normal numbers: the unit's estimate and one Newton step
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(m));
+  return fmaf(r, fmaf(-m, r, 1.f), r);
+}
+// (mean + eps)^(-1/2), likewise.
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = rsqrtf(v), half = 0.5f * r;
+  const float refined = fmaf(half, fmaf(-v * r, r, 1.f), r);
+  return v < __uint_as_float(0x7f800000u) ? refined : r;  // infinity: 0, not 0 * infinity
+}
 __device__ __forceinline__ float code_factor(float m, float rstd, float largest) {
   const float top = m * rstd;
   if (!(top < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);  // a NaN or an infinity: reads as NaN
-  return top >= kSmallestAmax ? largest / m : largest * rstd / kSmallestAmax;
+  return top >= kSmallestAmax ? largest * reciprocal(m) : largest * rstd * (1.f / kSmallestAmax);
 }
-__device__ __forceinline__ float code_scale(float m, float rstd, float largest) {
+__device__ __forceinline__ float code_scale(float m, float rstd, float inv_largest) {
   const float top = m * rstd;
-  return top < __uint_as_float(0x7f800000u) ? fmaxf(top, kSmallestAmax) / largest : __uint_as_float(0x7fffffffu);
+  return top < __uint_as_float(0x7f800000u) ? fmaxf(top, kSmallestAmax) * inv_largest : __uint_as_float(0x7fffffffu);
 }
 
 // One row for a block (TEAM 0), or RU rows for a team of TEAM lanes; rows that are read
@@ -232,10 +241,6 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
   __shared__ unsigned chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const long long first = (long long)blockIdx.x * blockDim.y * RU + threadIdx.y;
-  if (!TEAM) {
-    if (me < 64) slot[me >> 5][me & 31] = 0.f;
-    __syncthreads();
-  }
   uint4 h[RU][NV], r[RU][NV];
 #pragma unroll
   for (int u = 0; u < RU; ++u) {
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
   for (int u = 0; u < RU; ++u) {
     const long long row = first + u * blockDim.y;
-    rstd[u] = 1.f / sqrtf(sum[u] / (float)cols + p.eps);
+    rstd[u] = inverse_root(fmaf(sum[u], p.inv_cols, p.eps));
     if (me == 0 && row < p.rows) p.rstd[row] = rstd[u];
   }
 
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 
   // 8-bit codes.  Aligned rows: a group of at most 128 columns lies in neighbouring lanes of one warp.  Other rows: 32
   // columns lie in the lanes of a warp, and larger groups are put together in shared memory.
-  const float largest = largest_code(p.code);
+  const float largest = p.largest;
   const bool whole = p.groups == 1;
   float top[RU];
   if (whole || !VEC) {
@@ -354,7 +359,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         }
         if (c >= cols || row >= p.rows) continue;
         if (whole ? c == 0 : (c & ((1 << p.group_shift) - 1)) == 0)
-          p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = code_scale(m, rstd[u], largest);
+          p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = code_scale(m, rstd[u], p.inv_largest);
         const Pair f = twice(code_factor(m, rstd[u], largest));
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) a[e] = a[e] * f;
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
             for (int k = begin; k < end; ++k) bits = max(bits, chunk[threadIdx.y * 32 + k]);
             m = __uint_as_float(bits);
           }
-          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = code_scale(m, rstd[u], largest);
+          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = code_scale(m, rstd[u], p.inv_largest);
           const float v = e & 1 ? a[e / 2].get().y : a[e / 2].get().x;
           out[c] = (unsigned char)encode1(v * code_factor(m, rstd[u], largest), p.code);
         }
@@ -442,10 +447,6 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
   extern __shared__ __align__(16) float shared[];  // teams * cols floats
   __shared__ __align__(16) float slot[2][32];
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
-  if (!TEAM) {
-    if (me < 64) slot[me >> 5][me & 31] = 0.f;
-    __syncthreads();
-  }
   Pair acc[NV * E / 2];
 #pragma unroll
   for (int i = 0; i < NV * E / 2; ++i) acc[i] = twice(0.f);
@@ -526,10 +527,6 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
   __shared__ __align__(16) float slot[2][32];
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const int threads = blockDim.x * blockDim.y, place = threadIdx.y * blockDim.x + me;
-  if (!TEAM) {
-    for (int i = me; i < 64; i += blockDim.x) slot[i >> 5][i & 31] = 0.f;
-    __syncthreads();
-  }
   const long long step = (long long)gridDim.x * blockDim.y;
   auto fetch = [&](int stage, long long row) {
     uint4* to = ring + (size_t)stage * TENSORS * NV * threads + place;
@@ -778,6 +775,9 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
   p.weight_f32 = weight_dtype == DGN_F32;
   p.code = code;
   p.eps = eps;
+  p.inv_cols = 1.f / (float)cols;
+  p.largest = code == DGN_CODE_I8 ? 127.f : code == DGN_CODE_E4M3 ? 448.f : 57344.f;
+  p.inv_largest = 1.f / p.largest;
   const void* fn = dtype == DGN_F32   ? norm_kernel<float>(s, vec, code != 0)
                    : dtype == DGN_F16 ? norm_kernel<__half>(s, vec, code != 0)
                                       : norm_kernel<__nv_bfloat16>(s, vec, code != 0);
