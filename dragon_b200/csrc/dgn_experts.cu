@@ -52,22 +52,17 @@ __device__ __forceinline__ float value_of(unsigned order) {
   return __uint_as_float(order >> 31 ? order ^ 1u << 31 : ~order);
 }
 
-// Largest key of a warp and the lowest index that has it.
+// Largest key of a warp and the lowest index that has it, the halves of the key one after the other.
 __device__ __forceinline__ void first_largest(u64* key, int* index) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const u64 k = __shfl_xor_sync(kFull, *key, d);
-    const int i = __shfl_xor_sync(kFull, *index, d);
-    if (k > *key || (k == *key && i < *index)) {
-      *key = k;
-      *index = i;
-    }
-  }
+  const unsigned high = *key >> 32, most = __reduce_max_sync(kFull, high);
+  const unsigned low = high == most ? (unsigned)*key : 0, rest = __reduce_max_sync(kFull, low);
+  *index = __reduce_min_sync(kFull, high == most && low == rest ? (unsigned)*index : ~0u);
+  *key = (u64)most << 32 | rest;
 }
 
 // One token's choice in 64 bits by a whole warp, its keys in shared memory.  Taken by the
 // tokens whose choice hangs on values that float32 does not tell apart, and by those that
-// hold a NaN or an infinity: a few in a thousand, so it is made small, not fast.
+// hold a NaN or an infinity: about one in a thousand, but a small batch waits for that one.
 template <typename T>
 __device__ __noinline__ void route_exact(const RouteParams& p, long long token, double* key) {
   const int lane = threadIdx.x & 31, experts = p.experts;
@@ -78,6 +73,7 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
   for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
   const auto raised = [&](double l) { return isinf(l) && l < 0 ? 0.0 : exp(l - top); };
   if (!p.sigmoid) {
+#pragma unroll 4
     for (int e = lane; e < experts; e += 32) sum += raised(widen(row[e]));
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
@@ -86,49 +82,37 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
     const double l = widen(row[e]);
     return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : raised(l) / sum;
   };
+  // With groups whose values are sums of scores, the scores come first and the logits take their place.
+  const bool sums = p.groups > 1 && p.best == 2 && !p.bias;
   __syncwarp();
+#pragma unroll 4
   for (int e = lane; e < experts; e += 32) {
     const double l = widen(row[e]);
-    key[e] = p.bias && !(isinf(l) && l < 0) ? score(e) + (double)p.bias[e] : l;
+    if (isinf(l) && l < 0) key[e] = l;
+    else if (p.bias) key[e] = score(e) + (double)p.bias[e];
+    else key[e] = sums ? score(e) : l;
   }
   __syncwarp();
+  unsigned kept = ~0u;
+  const int width = experts / p.groups;
   if (p.groups > 1) {
-    const int width = experts / p.groups;
-    const bool by_key = p.bias || p.best == 1;  // otherwise the score is what is added up
-    u64 mine = 0;                               // lane g: the value of group g
-    for (int g = 0; g < p.groups; ++g) {
+    u64 mine = 0;  // lane g: the value of group g
+    if (lane < p.groups) {
       u64 a = 0, b = 0;  // the two largest, by order
-      int ia = kMaxExperts, ib = kMaxExperts;
       double va = 0.0, vb = 0.0;
-      for (int e = g * width + lane; e < (g + 1) * width; e += 32) {
-        if (!order_of(key[e])) continue;
-        const double v = by_key ? key[e] : score(e);
+      for (int i = 0; i < width; ++i) {
+        const double v = key[lane * width + (i + lane) % width];  // each lane at another bank
         const u64 o = order_of(v);
         if (o > a) {
-          b = a; ib = ia; vb = va;
-          a = o; ia = e; va = v;
+          b = a; vb = va;
+          a = o; va = v;
         } else if (o > b) {
-          b = o; ib = e; vb = v;
+          b = o; vb = v;
         }
       }
-      u64 k1 = a;
-      int i1 = ia;
-      first_largest(&k1, &i1);
-      if (p.best == 1 || !k1) {
-        if (lane == g) mine = k1;
-        continue;
-      }
-      const int owner1 = __ffs(__ballot_sync(kFull, a == k1 && ia == i1)) - 1;
-      const double v1 = __shfl_sync(kFull, va, owner1);
-      if (lane == owner1) { a = b; ia = ib; va = vb; }
-      u64 k2 = a;
-      int i2 = ia;
-      first_largest(&k2, &i2);
-      const int owner2 = __ffs(__ballot_sync(kFull, a == k2 && ia == i2)) - 1;
-      const double v2 = __shfl_sync(kFull, va, owner2);
-      if (lane == g) mine = order_of(k2 ? v1 + v2 : v1);
+      mine = p.best == 2 && b ? order_of(va + vb) : a;
     }
-    unsigned kept = 0;
+    kept = 0;
     for (int n = 0; n < p.keep; ++n) {
       u64 k1 = mine;
       int g = lane;
@@ -137,15 +121,17 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
       kept |= 1u << g;
       if (lane == g) mine = 0;
     }
-    __syncwarp();
-    for (int e = lane; e < experts; e += 32)
-      if (!(kept >> (e / width) & 1)) key[e] = -INFINITY;
-    __syncwarp();
+  }
+  __syncwarp();
+  for (int e = lane; e < experts; e += 32) {
+    if (!(kept >> (e * p.magic >> 20 & 31) & 1)) key[e] = -INFINITY;
+    else if (sums && !(isinf(key[e]) && key[e] < 0)) key[e] = widen(row[e]);
   }
   int index = -1;
   for (int n = 0; n < p.k; ++n) {
     u64 best = 0;
     int at = kMaxExperts;
+#pragma unroll 4
     for (int e = lane; e < experts; e += 32) {
       const u64 o = order_of(key[e]);
       if (o > best) {
@@ -157,7 +143,6 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
     if (!best) break;
     if (lane == n) index = at;
     if (lane == (at & 31)) key[at] = -INFINITY;
-    __syncwarp();
   }
   const float s = index < 0 ? 0.f : (float)score(index);
   float w = s;
@@ -173,13 +158,55 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
   }
 }
 
+// The k + 1 largest words of a token, put in the order of their keys in 64 bits: for a
+// choice between them that float32 does not decide.  All L lanes of each team of the warp
+// call it; `near`: whether this team's words need it.
+template <typename T, int L>
+__device__ __noinline__ void sort_exact(const RouteParams& p, const T* row, bool near, unsigned* win, double* key,
+                                        unsigned low) {
+  const int lane = threadIdx.x % L;
+  double top = -INFINITY, sum = 0.0;
+  if (p.bias && !p.sigmoid) {
+    for (int e = lane; e < p.experts; e += L) top = fmax(top, (double)widen(row[e]));
+#pragma unroll
+    for (int d = L / 2; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
+    for (int e = lane; near && e < p.experts; e += L) sum += exp((double)widen(row[e]) - top);  // -inf adds 0
+#pragma unroll
+    for (int d = L / 2; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+  }
+  for (int j = lane; near && j <= p.k; j += L) {
+    key[j] = -INFINITY;
+    if (!win[j]) continue;
+    const int e = low - (win[j] & low);
+    const double l = widen(row[e]);
+    key[j] = !p.bias ? l : (p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / sum) + (double)p.bias[e];
+  }
+  __syncwarp();
+  unsigned mine[kMaxChoices / L + 1];
+  int rank[kMaxChoices / L + 1];
+#pragma unroll
+  for (int q = 0; q <= kMaxChoices / L; ++q) {
+    const int j = q * L + lane;
+    rank[q] = -1;
+    if (!near || j > p.k || !win[j]) continue;
+    mine[q] = win[j];
+    rank[q] = 0;
+    for (int i = 0; i <= p.k; ++i)
+      rank[q] += win[i] && (key[i] > key[j] || (key[i] == key[j] && (win[i] & low) > (win[j] & low)));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q <= kMaxChoices / L; ++q)
+    if (rank[q] >= 0) win[rank[q]] = mine[q];
+  __syncwarp();
+}
+
 // exp(x) to about 2^-22 of its largest value in a row of differences to the maximum.
 __device__ __forceinline__ float quick_exp(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
   return r;
 }
-__device__ __forceinline__ float quick_sigmoid(float x) { return __fdividef(1.f, 1.f + quick_exp(-x)); }
 
 // N logits of a row for each of L lanes in float32, -inf behind the last.  VEC: 16 bytes
 // at a time, lane l has vectors l, l + L, ...; otherwise elements l, l + L, ...
@@ -229,13 +256,17 @@ template <int L> __device__ __forceinline__ unsigned team_max(unsigned v) {
 
 constexpr int kRouteThreads = 128;
 
-// Shared memory of one warp: its teams' keys by group, or the keys of route_exact; then each team's winners and group values.
+// Words of a team: its k + 2 winners, its groups' values, the keys of sort_exact.
+constexpr int kWinWords = 36, kTeamWords = kWinWords + kMaxGroups + 2 * (kMaxChoices + 2);
+static_assert(kWinWords >= kMaxChoices + 2 && kTeamWords % 4 == 0 && (kWinWords + kMaxGroups) % 2 == 0, "aligned parts");
+
+// Shared memory of one warp: its teams' keys by group, or the keys of route_exact; then the words of its teams.
 __host__ __device__ inline int route_values(int experts, int groups, int teams) {
   const int grouped = groups > 1 ? teams * (experts + groups) * 4 : 0;
   return (max(grouped, experts * 8) + 15) / 16 * 16;
 }
 __host__ __device__ inline int route_shared(int experts, int groups, int teams) {
-  return route_values(experts, groups, teams) + teams * (kMaxChoices + 1 + kMaxGroups + 3) * 4;
+  return route_values(experts, groups, teams) + teams * kTeamWords * 4;
 }
 
 // L lanes for a token, N experts for a lane; experts <= 1 << bits <= L * N.
@@ -245,9 +276,12 @@ __host__ __device__ inline int route_shared(int experts, int groups, int teams) 
 // one 31-bit word: the key's order without its lowest bits, which hold the number, the lowest
 // the largest.  So the words differ, one maximum finds value and place at once, and the
 // next largest is the largest of word - last, wrapped around, without anything being marked.
-// The choice stands if float32 tells each of the k + 1 first words from the next (by the
-// gap between what their upper bits leave open, less the rounding of the scores where there
-// is a bias); otherwise route_exact makes it again.  16-bit logits lose nothing with the lowest bits.
+// With a bias the upper bits are not the key's order but its distance from the row's largest
+// in even steps, as fine as the scores are exact.  The choice stands if each of the k + 1
+// first words is clear of the next: by what its upper bits leave open, and by the rounding of the
+// scores where there is a bias.  Otherwise sort_exact orders those k + 1, and where more than
+// they are too near the border, or a value is not finite, route_exact makes the whole choice.  16-bit
+// logits without a bias lose nothing with the lowest bits and need none of this.
 template <typename T, int L, int N, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteParams p) {
   constexpr int TEAMS = 32 / L;
@@ -256,8 +290,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x % L, team = (threadIdx.x & 31) / L, experts = p.experts;
   char* mine = shared + warp * route_shared(experts, p.groups, TEAMS);
   unsigned* win = reinterpret_cast<unsigned*>(mine + route_values(experts, p.groups, TEAMS)) +
-                  team * (kMaxChoices + 1 + kMaxGroups + 3);
-  float* group_value = reinterpret_cast<float*>(win + kMaxChoices + 1);
+                  team * kTeamWords;
+  float* group_value = reinterpret_cast<float*>(win + kWinWords);
+  double* exact_key = reinterpret_cast<double*>(group_value + kMaxGroups);
   const long long token = ((long long)blockIdx.x * (kRouteThreads / 32) + warp) * TEAMS + team;
   const bool live = token < p.tokens && !(p.mask && !p.mask[token]);
   const T* row = reinterpret_cast<const T*>(p.logits) + (live ? token : 0) * p.stride;
@@ -282,9 +317,18 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     for (int i = 0; i < N; ++i) sum[i & 3] += quick_exp(x[i] - top);
     inv = largest_score = 1.f / team_sum<L>((sum[0] + sum[1]) + (sum[2] + sum[3]));
   }
-  const auto quick_score = [&](float l) { return p.sigmoid ? quick_sigmoid(l) : quick_exp(l - top) * inv; };
-  // Twice what a score may be off by: 2^-22 of the largest for its exponential, 15 additions and a quotient at 2^-24.
-  const float slack = largest_score * 0x1p-18f;
+  const auto score_of = [&](float l) { return p.sigmoid ? __fdividef(1.f, 1.f + expf(-l)) : quick_exp(l - top) * inv; };
+  // Twice what a score may be off by.  Softmax: 2^-22 of the largest for its exponential, 15 additions and a quotient at
+  // 2^-24.  Sigmoid: two steps of expf weigh a quarter, then half a step of the sum and two of the quotient.
+  const float slack = largest_score * (p.sigmoid ? 0x1p-20f : 0x1p-18f);
+  if (p.bias) {  // from here on x is the key
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      if (x[i] > -INFINITY) x[i] = score_of(x[i]) + p.bias[e];
+      odd |= !(x[i] < INFINITY);
+    }
+  }
 
   unsigned kept = ~0u;
   const int width = experts / p.groups;
@@ -294,10 +338,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     for (int i = 0; i < N; ++i) {
       const int e = expert_of<T, L, VEC>(i, lane);
       if (e >= experts) continue;
-      const float v = x[i] == -INFINITY ? x[i]
-                      : p.bias          ? quick_score(x[i]) + p.bias[e]
-                      : p.best == 2     ? quick_score(x[i])
-                                        : x[i];
+      const float v = p.bias || p.best == 1 || x[i] == -INFINITY ? x[i] : score_of(x[i]);
       values[e + (e * p.magic >> 20)] = v;  // a word between the groups keeps them in different banks
     }
     __syncwarp();
@@ -333,22 +374,43 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     kept = bits;
     // Logits alone are compared as they are; sums and scores have to be further apart than they may be off.
     if ((p.bias || p.best == 2) && p.keep < p.groups && next > -INFINITY)
-      odd |= !(worst - next > 2.f * slack + 0x1p-20f * (fabsf(worst) + fabsf(next)));
+      odd |= !(worst - next > 2.f * slack + 0x1p-22f * (fabsf(worst) + fabsf(next)));
   }
 
-  unsigned word[N];
+  // Words: the upper bits of the key's order, or of its place between the largest and the smallest key.
+  unsigned word[N], need = 1;  // need: how many steps apart two words have to be
+  if (!p.bias) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = expert_of<T, L, VEC>(i, lane);
-    float v = x[i];
-    if (p.bias && e < experts && v > -INFINITY) {
-      v = quick_score(v) + p.bias[e];
-      odd |= !(v < INFINITY);
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      word[i] = x[i] > -INFINITY && (kept >> (e * p.magic >> 20 & 31) & 1) ? (order_of(x[i]) >> 1 & ~low) | (low - e) : 0;
     }
-    word[i] = v > -INFINITY && (kept >> (e * p.magic >> 20 & 31) & 1) ? (order_of(v) >> 1 & ~low) | (low - e) : 0;
+  } else {
+    float most = -INFINITY, least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      if (!(kept >> (e * p.magic >> 20 & 31) & 1)) x[i] = -INFINITY;
+      most = fmaxf(most, x[i]);
+      least = fminf(least, x[i] > -INFINITY ? x[i] : INFINITY);
+    }
+    most = team_max<L>(most);
+    least = -team_max<L>(-least);
+    const float steps = (float)((1 << min(23, 30 - p.bits)) - 1);
+    const float range = fminf(most - least, 64.f * largest_score), base = most - range;  // far below: one step holds them all
+    const float scale = range > 0.f ? steps / range : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = expert_of<T, L, VEC>(i, lane);
+      const unsigned step = 1 + (unsigned)fminf(fmaxf((x[i] - base) * scale, 0.f), steps);
+      word[i] = x[i] > -INFINITY ? step << p.bits | (low - e) : 0;
+    }
+    // The place's own rounding is below two steps for each of two words; keys are off by half the slack and their rounding.
+    need = 5 + (unsigned)fminf((slack + 0x1p-22f * fmaxf(fabsf(most), fabsf(base))) * scale, 1e6f);
   }
   unsigned last = kWrap;
-  const int wanted = p.k + (sizeof(T) == 2 && !p.bias ? 0 : 1);
+  const bool certain = sizeof(T) == 2 && !p.bias;
+  const int wanted = p.k + (certain ? 0 : 2);
   for (int j = 0; j < wanted; ++j) {
     unsigned best = 0;
 #pragma unroll
@@ -359,6 +421,23 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     if (last == 0) last = 1;  // nothing is left: only zeros stay below
   }
   __syncwarp();
+  if (!certain) {
+    bool near = false;
+    for (int j = lane; j < p.k; j += L) {
+      const unsigned a = win[j], b = win[j + 1];
+      if (!b || (a >> p.bits) - (b >> p.bits) >= need) continue;
+      // Two experts with the same logit and bias are in order; at the border there may be more of them.
+      const int e = low - (a & low), f = low - (b & low);
+      near |= j + 1 == p.k || widen(row[e]) != widen(row[f]) || (p.bias && p.bias[e] != p.bias[f]);
+    }
+    const unsigned team_lanes = L == 32 ? ~0u : ((1u << (L & 31)) - 1) << (team * L);
+    const unsigned all = __ballot_sync(kFull, near && live);
+    if (all) {
+      near = all & team_lanes;
+      if (near && win[p.k + 1]) odd |= (win[p.k - 1] >> p.bits) - (win[p.k + 1] >> p.bits) < need;
+      sort_exact<T, L>(p, row, near, win, exact_key, low);
+    }
+  }
 
   // Choice j belongs to lane j % L.
   float score[kMaxChoices / L];
@@ -375,18 +454,6 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     const float l = widen(row[index[q]]);
     score[q] = p.sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - first) * inv;
     total += score[q];
-    const unsigned after = j + 1 < wanted ? win[j + 1] : 0;
-    if (!after) continue;
-    if (!p.bias) {
-      odd |= sizeof(T) == 4 && (win[j] & ~low) == (after & ~low);
-    } else {
-      const float floor = value_of((win[j] & ~low) << 1), ceiling = value_of(((after | low) + 1) << 1);
-      if (!(floor - ceiling > slack + 0x1p-21f * fabsf(floor))) {
-        // Two experts with the same logit and bias are in order; behind the last choice there may be more to see.
-        const int other = low - (after & low);
-        odd |= j + 1 == p.k || widen(row[other]) != l || p.bias[other] != p.bias[index[q]];
-      }
-    }
   }
   total = p.renormalize ? team_sum<L>(total) + kTiny : 1.f;
   const unsigned again = __ballot_sync(kFull, odd && live);
