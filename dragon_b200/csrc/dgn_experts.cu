@@ -33,6 +33,7 @@ struct RouteParams {
   int experts, k, sigmoid, groups, keep, best, renormalize;
   int bits;        // of an expert's number
   unsigned magic;  // e * magic >> 20 is expert e's group
+  int group_lanes; // lanes whose vectors make up a group; 0: not a power of two of them in one team
   float scale;
 };
 
@@ -43,13 +44,10 @@ __device__ __forceinline__ u64 order_of(double v) {
   const u64 bits = (u64)__double_as_longlong(v + 0.0);  // -0 becomes 0
   return bits >> 63 ? ~bits : bits | 1ull << 63;
 }
-// The same for float32, and back.
+// The same for float32, -inf and NaN left aside.
 __device__ __forceinline__ unsigned order_of(float v) {
-  const unsigned bits = __float_as_uint(v + 0.f);
-  return bits >> 31 ? ~bits : bits | 1u << 31;
-}
-__device__ __forceinline__ float value_of(unsigned order) {
-  return __uint_as_float(order >> 31 ? order ^ 1u << 31 : ~order);
+  const int bits = __float_as_int(v + 0.f);
+  return bits ^ (bits >> 31 | 1 << 31);
 }
 
 // Largest key of a warp and the lowest index that has it, the halves of the key one after the other.
@@ -208,31 +206,39 @@ __device__ __forceinline__ float quick_exp(float x) {
   return r;
 }
 
-// N logits of a row for each of L lanes in float32, -inf behind the last.  VEC: 16 bytes
-// at a time, lane l has vectors l, l + L, ...; otherwise elements l, l + L, ...
+__device__ __forceinline__ float quick_reciprocal(float x) {  // to one step
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// N values of a row for each of L lanes in float32, -inf behind the last.  VEC: V neighbours
+// (16 bytes of the logits) at a time, lane l has the vectors l, l + L, ...; otherwise elements l, l + L, ...
 template <typename T, int L, bool VEC>
 __device__ __forceinline__ int expert_of(int i, int lane) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   return (i / V * L + lane) * V + i % V;
 }
-template <typename T, int L, int N, bool VEC>
+template <typename T, int L, int N, bool VEC, int V = 16 / (int)sizeof(T)>
 __device__ __forceinline__ void load_logits(const T* row, bool live, int experts, int lane, float* x) {
   if constexpr (VEC) {
-    constexpr int V = 16 / (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < N; i += V) {
-      const int e = expert_of<T, L, VEC>(i, lane);
-      if (live && e < experts) {
-        Elem<T>::unpack(*reinterpret_cast<const uint4*>(row + e), x + i);
-      } else {
+      const int e = (i / V * L + lane) * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[i + j] = -INFINITY;
+      for (int j = 0; j < V; j += Elem<T>::E) {
+        if (live && e < experts) {
+          Elem<T>::unpack(*reinterpret_cast<const uint4*>(row + e + j), x + i + j);
+        } else {
+#pragma unroll
+          for (int n = 0; n < Elem<T>::E; ++n) x[i + j + n] = -INFINITY;
+        }
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = expert_of<T, L, VEC>(i, lane);
+      const int e = i * L + lane;
       x[i] = live && e < experts ? widen(row[e]) : -INFINITY;
     }
   }
@@ -317,61 +323,107 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     for (int i = 0; i < N; ++i) sum[i & 3] += quick_exp(x[i] - top);
     inv = largest_score = 1.f / team_sum<L>((sum[0] + sum[1]) + (sum[2] + sum[3]));
   }
-  const auto score_of = [&](float l) { return p.sigmoid ? __fdividef(1.f, 1.f + expf(-l)) : quick_exp(l - top) * inv; };
+  const auto score_of = [&](float l) { return p.sigmoid ? quick_reciprocal(1.f + quick_exp(-l)) : quick_exp(l - top) * inv; };
   // Twice what a score may be off by.  Softmax: 2^-22 of the largest for its exponential, 15 additions and a quotient at
-  // 2^-24.  Sigmoid: two steps of expf weigh a quarter, then half a step of the sum and two of the quotient.
+  // 2^-24.  Sigmoid: its exponential's error weighs s (1 - s), 2^-24 with |l| at its worst; then half a step of the sum
+  // and one of the reciprocal.
   const float slack = largest_score * (p.sigmoid ? 0x1p-20f : 0x1p-18f);
   if (p.bias) {  // from here on x is the key
+    float b[N];
+    load_logits<float, L, N, VEC, 16 / (int)sizeof(T)>(p.bias, live, experts, lane, b);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = expert_of<T, L, VEC>(i, lane);
-      if (x[i] > -INFINITY) x[i] = score_of(x[i]) + p.bias[e];
+      if (x[i] > -INFINITY) x[i] = score_of(x[i]) + b[i];
       odd |= !(x[i] < INFINITY);
     }
   }
 
-  unsigned kept = ~0u;
-  const int width = experts / p.groups;
   if (p.groups > 1) {
-    float* values = reinterpret_cast<float*>(mine) + team * (experts + p.groups);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = expert_of<T, L, VEC>(i, lane);
-      if (e >= experts) continue;
-      const float v = p.bias || p.best == 1 || x[i] == -INFINITY ? x[i] : score_of(x[i]);
-      values[e + (e * p.magic >> 20)] = v;  // a word between the groups keeps them in different banks
-    }
-    __syncwarp();
-    for (int g = lane; g < p.groups; g += L) {
-      float a = -INFINITY, b = -INFINITY;
-      for (int i = 0; i < width; ++i) {
-        const float v = values[g * (width + 1) + i];
-        b = fmaxf(b, fminf(a, v));
-        a = fmaxf(a, v);
-      }
-      group_value[g] = p.best == 2 && b > -INFINITY ? a + b : a;
-    }
-    __syncwarp();
-    unsigned bits = 0;
     float worst = INFINITY, next = -INFINITY;  // the values on either side of the border
-    for (int g = lane; g < p.groups; g += L) {
-      const float v = group_value[g];
-      int rank = 0;
-      for (int o = 0; o < p.groups; ++o) rank += group_value[o] > v || (group_value[o] == v && o < g);
-      if (rank < p.keep) {
-        bits |= 1u << g;
-        worst = fminf(worst, v);
-      } else {
-        next = fmaxf(next, v);
-      }
-    }
+    if (VEC && p.group_lanes) {
+      // A group is p.group_lanes neighbouring lanes' vectors: its value is made and compared in registers.
+      constexpr int V = 16 / (int)sizeof(T), C = VEC ? N / V : 1;
+      float value[C];
 #pragma unroll
-    for (int d = L / 2; d; d >>= 1) {
-      bits |= __shfl_xor_sync(kFull, bits, d);
-      worst = fminf(worst, __shfl_xor_sync(kFull, worst, d));
-      next = fmaxf(next, __shfl_xor_sync(kFull, next, d));
+      for (int c = 0; c < C; ++c) {
+        float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float l = x[c * V + i], v = p.bias || p.best == 1 || l == -INFINITY ? l : score_of(l);
+          b = fmaxf(b, fminf(a, v));
+          a = fmaxf(a, v);
+        }
+        for (int d = p.group_lanes / 2; d; d >>= 1) {
+          const float oa = __shfl_xor_sync(kFull, a, d), ob = __shfl_xor_sync(kFull, b, d);
+          b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+          a = fmaxf(a, oa);
+        }
+        value[c] = p.best == 2 && b > -INFINITY ? a + b : a;
+      }
+      int rank[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) rank[c] = 0;
+#pragma unroll
+      for (int o = 0; o < C; ++o)
+        for (int from = 0; from < L; from += p.group_lanes) {
+          const float other = __shfl_sync(kFull, value[o], team * L + from);
+#pragma unroll
+          for (int c = 0; c < C; ++c)  // equal ones: the earlier
+            rank[c] += other > value[c] || (other == value[c] && (o < c || (o == c && from + p.group_lanes <= lane)));
+        }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const bool there = expert_of<T, L, VEC>(c * V, lane) < experts;
+        if (rank[c] < p.keep) {
+          if (there) worst = fminf(worst, value[c]);
+        } else {
+          next = fmaxf(next, value[c]);
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[c * V + i] = -INFINITY;
+        }
+      }
+    } else {
+      const int width = experts / p.groups;
+      float* values = reinterpret_cast<float*>(mine) + team * (experts + p.groups);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = expert_of<T, L, VEC>(i, lane);
+        if (e >= experts) continue;
+        const float v = p.bias || p.best == 1 || x[i] == -INFINITY ? x[i] : score_of(x[i]);
+        values[e + (e * p.magic >> 20)] = v;  // a word between the groups keeps them in different banks
+      }
+      __syncwarp();
+      for (int g = lane; g < p.groups; g += L) {
+        float a = -INFINITY, b = -INFINITY;
+#pragma unroll 8
+        for (int i = 0; i < width; ++i) {
+          const float v = values[g * (width + 1) + i];
+          b = fmaxf(b, fminf(a, v));
+          a = fmaxf(a, v);
+        }
+        group_value[g] = p.best == 2 && b > -INFINITY ? a + b : a;
+      }
+      __syncwarp();
+      unsigned kept = 0;
+      for (int g = lane; g < p.groups; g += L) {
+        const float v = group_value[g];
+        int rank = 0;
+        for (int o = 0; o < p.groups; ++o) rank += group_value[o] > v || (group_value[o] == v && o < g);
+        if (rank < p.keep) {
+          kept |= 1u << g;
+          worst = fminf(worst, v);
+        } else {
+          next = fmaxf(next, v);
+        }
+      }
+#pragma unroll
+      for (int d = L / 2; d; d >>= 1) kept |= __shfl_xor_sync(kFull, kept, d);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!(kept >> (expert_of<T, L, VEC>(i, lane) * p.magic >> 20 & 31) & 1)) x[i] = -INFINITY;
     }
-    kept = bits;
+    worst = -team_max<L>(-worst);
+    next = team_max<L>(next);
     // Logits alone are compared as they are; sums and scores have to be further apart than they may be off.
     if ((p.bias || p.best == 2) && p.keep < p.groups && next > -INFINITY)
       odd |= !(worst - next > 2.f * slack + 0x1p-22f * (fabsf(worst) + fabsf(next)));
@@ -383,14 +435,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = expert_of<T, L, VEC>(i, lane);
-      word[i] = x[i] > -INFINITY && (kept >> (e * p.magic >> 20 & 31) & 1) ? (order_of(x[i]) >> 1 & ~low) | (low - e) : 0;
+      word[i] = x[i] > -INFINITY ? (order_of(x[i]) >> 1 & ~low) | (low - e) : 0;
     }
   } else {
     float most = -INFINITY, least = INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = expert_of<T, L, VEC>(i, lane);
-      if (!(kept >> (e * p.magic >> 20 & 31) & 1)) x[i] = -INFINITY;
       most = fmaxf(most, x[i]);
       least = fminf(least, x[i] > -INFINITY ? x[i] : INFINITY);
     }
@@ -414,7 +464,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   for (int j = 0; j < wanted; ++j) {
     unsigned best = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = max(best, word[i] - last);
+    for (int i = 0; i < N; ++i) best = __viaddmax_u32(word[i], -last, best);
     best = best >= kWrap ? best + last : 0;
     last = team_max<L>(best);
     if (lane == j % L) win[j] = last;
@@ -449,6 +499,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     const int j = q * L + lane;
     index[q] = -1;
     score[q] = 0.f;
+    if (q * L >= p.k) break;
     if (j >= p.k || !win[j]) continue;
     index[q] = low - (win[j] & low);
     const float l = widen(row[index[q]]);
@@ -462,7 +513,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 #pragma unroll
     for (int q = 0; q < kMaxChoices / L; ++q) {
       const int j = q * L + lane;
-      if (j >= p.k) continue;
+      if (j >= p.k) break;
       p.indices[token * p.k + j] = index[q];
       p.weights[token * p.k + j] = index[q] < 0 ? 0.f : (p.renormalize ? score[q] / total : score[q]) * p.scale;
     }
@@ -968,7 +1019,9 @@ extern "C" int dgn_route(const void* logits, int64_t stride, const float* bias, 
   while (1 << p.bits < experts) ++p.bits;
   p.magic = (unsigned)ceil_div(1 << 20, experts / groups);
   const int elems = 16 / (int)dgn_dtype_size(dtype), teams = 32 / route_lanes(experts);
-  const bool vec = experts % elems == 0 && stride % elems == 0 && aligned(logits, 16);
+  const bool vec = experts % elems == 0 && stride % elems == 0 && aligned(logits, 16) && aligned(bias, 16);
+  const int width = experts / groups, run = width / elems;
+  p.group_lanes = vec && width % elems == 0 && (run & (run - 1)) == 0 && run <= 32 / teams ? run : 0;
   const void* fn = dtype == DGN_F32   ? (vec ? route_fn<float, true>(experts) : route_fn<float, false>(experts))
                    : dtype == DGN_F16 ? (vec ? route_fn<__half, true>(experts) : route_fn<__half, false>(experts))
                    : vec              ? route_fn<__nv_bfloat16, true>(experts)
