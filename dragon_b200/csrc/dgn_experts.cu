@@ -37,12 +37,16 @@ struct RouteParams {
   float scale;
 };
 
-// Keys as whole numbers that sort like the values: 0 is "not to be chosen", NaN comes first.
+// Keys as whole numbers that sort like the values: 0 is "not to be chosen" (-inf), NaN comes first.
 __device__ __forceinline__ u64 order_of(double v) {
-  if (isnan(v)) return ~0ull;
-  if (isinf(v) && v < 0) return 0;
-  const u64 bits = (u64)__double_as_longlong(v + 0.0);  // -0 becomes 0
+  u64 bits = (u64)__double_as_longlong(v);
+  if (bits << 1 > 0xffe0000000000000ull) return ~0ull;  // NaN
+  if (bits == 0xfff0000000000000ull) return 0;           // -inf
+  if (bits == 1ull << 63) bits = 0;                      // -0
   return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+__device__ __forceinline__ double value_of(u64 order) {  // of any key but 0
+  return __longlong_as_double((long long)(order >> 63 ? order ^ 1ull << 63 : ~order));
 }
 // The same for float32, -inf and NaN left aside.
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -58,59 +62,77 @@ __device__ __forceinline__ void first_largest(u64* key, int* index) {
   *key = (u64)most << 32 | rest;
 }
 
-// One token's choice in 64 bits by a whole warp, its keys in shared memory.  Taken by the
+// Scores of four logits in 64 bits; `over` is the softmax's sum (0: its terms are wanted alone).  One copy for all kernels:
+// the few warps that take an exact path wait for its instructions to arrive, and for one value after the other unless
+// several are under way.
+__device__ __noinline__ void exact_scores(double* v, int sigmoid, double top, double over) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double e = exp(sigmoid ? -v[i] : v[i] - top);
+    v[i] = sigmoid ? 1.0 / (1.0 + e) : over != 0.0 ? e / over : e;
+  }
+}
+
+// One token's choice in 64 bits by a whole warp, its keys' orders in shared memory.  Taken by the
 // tokens whose choice hangs on values that float32 does not tell apart, and by those that
 // hold a NaN or an infinity: about one in a thousand, but a small batch waits for that one.
 template <typename T>
-__device__ __noinline__ void route_exact(const RouteParams& p, long long token, double* key) {
+__device__ __noinline__ void route_exact(const RouteParams& p, long long token, u64* key) {
   const int lane = threadIdx.x & 31, experts = p.experts;
   const T* row = reinterpret_cast<const T*>(p.logits) + token * p.stride;
-  double top = -INFINITY, sum = 0.0;
-  for (int e = lane; e < experts; e += 32) top = fmax(top, (double)widen(row[e]));
+  // With groups whose values are sums of scores, the scores come first and the logits take their place.
+  const bool sums = p.groups > 1 && p.best == 2 && !p.bias;
+  float top = -INFINITY;
+  for (int e = lane; e < experts; e += 32) top = fmaxf(top, widen(row[e]));
 #pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
-  const auto raised = [&](double l) { return isinf(l) && l < 0 ? 0.0 : exp(l - top); };
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+  double sum = 0.0;
   if (!p.sigmoid) {
-#pragma unroll 4
-    for (int e = lane; e < experts; e += 32) sum += raised(widen(row[e]));
+#pragma unroll 1
+    for (int base = lane; base < experts; base += 128) {
+      double v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = base + i * 32 < experts ? (double)widen(row[base + i * 32]) : -INFINITY;
+      exact_scores(v, 0, top, 0.0);  // -inf gives 0
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
   }
-  const auto score = [&](int e) {
-    const double l = widen(row[e]);
-    return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : raised(l) / sum;
-  };
-  // With groups whose values are sums of scores, the scores come first and the logits take their place.
-  const bool sums = p.groups > 1 && p.best == 2 && !p.bias;
   __syncwarp();
-#pragma unroll 4
-  for (int e = lane; e < experts; e += 32) {
-    const double l = widen(row[e]);
-    if (isinf(l) && l < 0) key[e] = l;
-    else if (p.bias) key[e] = score(e) + (double)p.bias[e];
-    else key[e] = sums ? score(e) : l;
+#pragma unroll 1
+  for (int base = lane; base < experts; base += 128) {
+    double v[4];
+    bool none[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = base + i * 32 < experts ? (double)widen(row[base + i * 32]) : -INFINITY;
+      none[i] = (float)v[i] == -INFINITY;
+    }
+    if (p.bias || sums) exact_scores(v, p.sigmoid, top, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = base + i * 32;
+      if (e < experts) key[e] = none[i] ? 0 : order_of(p.bias ? v[i] + (double)p.bias[e] : v[i]);
+    }
   }
   __syncwarp();
-  unsigned kept = ~0u;
-  const int width = experts / p.groups;
   if (p.groups > 1) {
+    const int width = experts / p.groups;
     u64 mine = 0;  // lane g: the value of group g
     if (lane < p.groups) {
-      u64 a = 0, b = 0;  // the two largest, by order
-      double va = 0.0, vb = 0.0;
+      u64 a = 0, b = 0;  // the two largest
+      const int turn = lane % width;  // each lane begins at another bank
+#pragma unroll 4
       for (int i = 0; i < width; ++i) {
-        const double v = key[lane * width + (i + lane) % width];  // each lane at another bank
-        const u64 o = order_of(v);
-        if (o > a) {
-          b = a; vb = va;
-          a = o; va = v;
-        } else if (o > b) {
-          b = o; vb = v;
-        }
+        const int at = i + turn;
+        const u64 o = key[lane * width + (at < width ? at : at - width)];
+        b = max(b, min(a, o));
+        a = max(a, o);
       }
-      mine = p.best == 2 && b ? order_of(va + vb) : a;
+      mine = p.best == 2 && b ? order_of(value_of(a) + value_of(b)) : a;
     }
-    kept = 0;
+    unsigned kept = 0;
     for (int n = 0; n < p.keep; ++n) {
       u64 k1 = mine;
       int g = lane;
@@ -119,11 +141,11 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
       kept |= 1u << g;
       if (lane == g) mine = 0;
     }
-  }
-  __syncwarp();
-  for (int e = lane; e < experts; e += 32) {
-    if (!(kept >> (e * p.magic >> 20 & 31) & 1)) key[e] = -INFINITY;
-    else if (sums && !(isinf(key[e]) && key[e] < 0)) key[e] = widen(row[e]);
+    __syncwarp();
+    for (int e = lane; e < experts; e += 32) {
+      if (!(kept >> (e * p.magic >> 20 & 31) & 1)) key[e] = 0;
+      else if (sums && key[e]) key[e] = order_of((double)widen(row[e]));
+    }
   }
   int index = -1;
   for (int n = 0; n < p.k; ++n) {
@@ -131,7 +153,7 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
     int at = kMaxExperts;
 #pragma unroll 4
     for (int e = lane; e < experts; e += 32) {
-      const u64 o = order_of(key[e]);
+      const u64 o = key[e];
       if (o > best) {
         best = o;
         at = e;
@@ -140,9 +162,13 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
     first_largest(&best, &at);
     if (!best) break;
     if (lane == n) index = at;
-    if (lane == (at & 31)) key[at] = -INFINITY;
+    if (lane == (at & 31)) key[at] = 0;
   }
-  const float s = index < 0 ? 0.f : (float)score(index);
+  float s = 0.f;
+  if (index >= 0) {
+    const float l = widen(row[index]);
+    s = p.sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - top) / (float)sum;
+  }
   float w = s;
   if (p.renormalize) {
     float total = s;
@@ -160,24 +186,40 @@ __device__ __noinline__ void route_exact(const RouteParams& p, long long token, 
 // choice between them that float32 does not decide.  All L lanes of each team of the warp
 // call it; `near`: whether this team's words need it.
 template <typename T, int L>
-__device__ __noinline__ void sort_exact(const RouteParams& p, const T* row, bool near, unsigned* win, double* key,
+__device__ __noinline__ void sort_exact(const RouteParams& p, const T* row, bool near, unsigned* win, u64* key,
                                         unsigned low) {
   const int lane = threadIdx.x % L;
-  double top = -INFINITY, sum = 0.0;
+  float top = -INFINITY;
+  double sum = 0.0;
   if (p.bias && !p.sigmoid) {
-    for (int e = lane; e < p.experts; e += L) top = fmax(top, (double)widen(row[e]));
+    for (int e = lane; e < p.experts; e += L) top = fmaxf(top, widen(row[e]));
 #pragma unroll
-    for (int d = L / 2; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, d));
-    for (int e = lane; near && e < p.experts; e += L) sum += exp((double)widen(row[e]) - top);  // -inf adds 0
+    for (int d = L / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+#pragma unroll 1
+    for (int base = lane; near && base < p.experts; base += 4 * L) {
+      double v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = base + i * L < p.experts ? (double)widen(row[base + i * L]) : -INFINITY;
+      exact_scores(v, 0, top, 0.0);  // -inf gives 0
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
 #pragma unroll
     for (int d = L / 2; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
   }
-  for (int j = lane; near && j <= p.k; j += L) {
-    key[j] = -INFINITY;
-    if (!win[j]) continue;
-    const int e = low - (win[j] & low);
-    const double l = widen(row[e]);
-    key[j] = !p.bias ? l : (p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / sum) + (double)p.bias[e];
+#pragma unroll 1
+  for (int base = lane; near && base <= p.k; base += 4 * L) {
+    double v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = base + i * L;
+      v[i] = j <= p.k && win[j] ? (double)widen(row[low - (win[j] & low)]) : 0.0;
+    }
+    if (p.bias) exact_scores(v, p.sigmoid, top, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = base + i * L;
+      if (j <= p.k) key[j] = !win[j] ? 0 : order_of(p.bias ? v[i] + (double)p.bias[low - (win[j] & low)] : v[i]);
+    }
   }
   __syncwarp();
   unsigned mine[kMaxChoices / L + 1];
@@ -189,6 +231,7 @@ __device__ __noinline__ void sort_exact(const RouteParams& p, const T* row, bool
     if (!near || j > p.k || !win[j]) continue;
     mine[q] = win[j];
     rank[q] = 0;
+#pragma unroll 1
     for (int i = 0; i <= p.k; ++i)
       rank[q] += win[i] && (key[i] > key[j] || (key[i] == key[j] && (win[i] & low) > (win[j] & low)));
   }
@@ -298,7 +341,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   unsigned* win = reinterpret_cast<unsigned*>(mine + route_values(experts, p.groups, TEAMS)) +
                   team * kTeamWords;
   float* group_value = reinterpret_cast<float*>(win + kWinWords);
-  double* exact_key = reinterpret_cast<double*>(group_value + kMaxGroups);
+  u64* exact_key = reinterpret_cast<u64*>(group_value + kMaxGroups);
   const long long token = ((long long)blockIdx.x * (kRouteThreads / 32) + warp) * TEAMS + team;
   const bool live = token < p.tokens && !(p.mask && !p.mask[token]);
   const T* row = reinterpret_cast<const T*>(p.logits) + (live ? token : 0) * p.stride;
@@ -452,8 +495,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = expert_of<T, L, VEC>(i, lane);
-      const unsigned step = 1 + (unsigned)fminf(fmaxf((x[i] - base) * scale, 0.f), steps);
-      word[i] = x[i] > -INFINITY ? step << p.bits | (low - e) : 0;
+      // 2^23 + step as a float32 has the step in its lowest bits: no conversion.
+      const float step = fminf(fmaxf(fmaf(x[i] - base, scale, 0x1p23f), 0x1p23f), 0x1p23f + steps);
+      word[i] = x[i] > -INFINITY ? (__float_as_uint(step) - 0x4affffffu) << p.bits | (low - e) : 0;
     }
     // The place's own rounding is below two steps for each of two words; keys are off by half the slack and their rounding.
     need = 5 + (unsigned)fminf((slack + 0x1p-22f * fmaxf(fabsf(most), fabsf(base))) * scale, 1e6f);
@@ -522,7 +566,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 #pragma unroll 1
   for (int t = 0; t < TEAMS; ++t)
     if (again & (L == 32 ? ~0u : ((1u << (L & 31)) - 1) << (t * L)))
-      route_exact<T>(p, token - team + t, reinterpret_cast<double*>(mine));
+      route_exact<T>(p, token - team + t, reinterpret_cast<u64*>(mine));
 }
 
 struct RouteGradParams {
