@@ -16,6 +16,7 @@ using namespace dgn;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChoices = 32;  // one lane of a warp for each
 constexpr int kMaxGroups = 32;
+constexpr int64_t kMaxRow = 1 << 30;  // so that a column plus a block's width stays a 32-bit number
 constexpr float kTiny = 1e-20f;  // keeps the sum that weights are divided by from zero
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -798,6 +799,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
 
 // ---- moves -----------------------------------------------------------------------------------
 
+constexpr int kMoveThreads = 256;
+
 struct MoveParams {
   const char* x;
   const int* positions;
@@ -808,31 +811,81 @@ struct MoveParams {
   int k, experts;
 };
 
-// Zeros in the rows of an expert's block that no slot uses.
+// Zeros in the rows of an expert's block that no slot uses, by a whole block of threads.
+// Such blocks come first in the grid: behind the others they would be its tail.
 template <typename U>
 __device__ void clear_rows(char* out, const int* counts, const int* offsets, int e, long long row_bytes,
                            long long capacity) {
   const long long first = max(0ll, (long long)offsets[e] + counts[e]), last = min((long long)offsets[e + 1], capacity);
-  const long long n = row_bytes / (long long)sizeof(U);
-  for (long long r = first; r < last; ++r)
-    for (long long i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<U*>(out + r * row_bytes)[i] = U{};
+  if (first >= last) return;
+  U* to = reinterpret_cast<U*>(out + first * row_bytes);
+  const long long n = (last - first) * row_bytes / (long long)sizeof(U);
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < n; i += kMoveThreads) to[i] = U{};
 }
 
-// A block for a token, then one for each expert's unused rows.
-template <typename U>
-__global__ void __launch_bounds__(256) dispatch_kernel(const __grid_constant__ MoveParams p) {
-  if (blockIdx.x >= p.tokens) {
-    clear_rows<U>(p.out, p.counts, p.offsets, (int)(blockIdx.x - p.tokens), p.row_bytes, p.capacity);
+// TEAM threads for a token: four words of its row at a time are read once and written to
+// each of its k places.
+template <typename U, int TEAM>
+__global__ void __launch_bounds__(kMoveThreads) dispatch_kernel(const __grid_constant__ MoveParams p) {
+  if (blockIdx.x < p.experts) {
+    clear_rows<U>(p.out, p.counts, p.offsets, blockIdx.x, p.row_bytes, p.capacity);
     return;
   }
-  const long long t = blockIdx.x;
+  __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
+  const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
+  const long long t = (long long)(blockIdx.x - p.experts) * (kMoveThreads / TEAM) + team;
+  if (t < p.tokens && me < p.k) place[team][me] = p.positions[t * p.k + me];
+  if (TEAM > 32) __syncthreads();
+  else __syncwarp();
+  if (t >= p.tokens) return;
   const U* from = reinterpret_cast<const U*>(p.x + t * p.x_stride);
   const long long n = p.row_bytes / (long long)sizeof(U);
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) {
-    const U v = from[i];
+  for (long long base = me; base < n; base += 4 * TEAM) {
+    U v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (base + i * TEAM < n) v[i] = from[base + i * TEAM];
     for (int j = 0; j < p.k; ++j) {
-      const long long at = p.positions[t * p.k + j];
-      if (at >= 0 && at < p.capacity) reinterpret_cast<U*>(p.out + at * p.row_bytes)[i] = v;
+      const int at = place[team][j];
+      if (at < 0 || at >= p.capacity) continue;
+      U* to = reinterpret_cast<U*>(p.out + at * p.row_bytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (base + i * TEAM < n) to[base + i * TEAM] = v[i];
+    }
+  }
+}
+
+// Part i of a row for thread `me` of TEAM: an aligned vector, or E elements TEAM apart so that
+// neighbouring threads still read neighbouring elements.
+template <typename T, bool VEC, int TEAM>
+__device__ __forceinline__ uint4 part(const char* row, int i, int me, int cols) {
+  constexpr int E = Elem<T>::E;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (VEC) {
+    const int c = (i * TEAM + me) * E;
+    if (c < cols) v = *reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T));
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = (i * E + e) * TEAM + me;
+      if (c < cols) reinterpret_cast<T*>(&v)[e] = reinterpret_cast<const T*>(row)[c];
+    }
+  }
+  return v;
+}
+template <typename T, bool VEC, int TEAM>
+__device__ __forceinline__ void put(char* row, int i, int me, int cols, uint4 v) {
+  constexpr int E = Elem<T>::E;
+  if (VEC) {
+    const int c = (i * TEAM + me) * E;
+    if (c < cols) *reinterpret_cast<uint4*>(row + (size_t)c * sizeof(T)) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = (i * E + e) * TEAM + me;
+      if (c < cols) reinterpret_cast<T*>(row)[c] = reinterpret_cast<const T*>(&v)[e];
     }
   }
 }
@@ -843,53 +896,54 @@ struct CombineParams {
   const float* weights;
   const char* residual;
   char* out;
-  long long tokens, cols, capacity, residual_stride;
-  int k;
+  long long tokens, capacity, residual_stride;
+  int cols, k;
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ uint4 part(const char* row, long long c, long long cols) {
-  if (VEC) return *reinterpret_cast<const uint4*>(row + c * (long long)sizeof(T));
-  uint4 v = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int i = 0; i < Elem<T>::E; ++i)
-    if (c + i < cols) reinterpret_cast<T*>(&v)[i] = reinterpret_cast<const T*>(row)[c + i];
-  return v;
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void put(char* row, long long c, long long cols, uint4 v) {
-  if (VEC) {
-    *reinterpret_cast<uint4*>(row + c * (long long)sizeof(T)) = v;
-    return;
+// TEAM threads for a token; four of its rows are on their way at a time.
+template <typename T, bool VEC, int TEAM>
+__global__ void __launch_bounds__(kMoveThreads) combine_kernel(const __grid_constant__ CombineParams p) {
+  constexpr int E = Elem<T>::E, AHEAD = 4;
+  __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
+  __shared__ float weight[kMoveThreads / TEAM][kMaxChoices];
+  const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
+  const long long t = (long long)blockIdx.x * (kMoveThreads / TEAM) + team, row_bytes = p.cols * (long long)sizeof(T);
+  if (t < p.tokens && me < p.k) {
+    const int at = p.positions[t * p.k + me];
+    place[team][me] = at < p.capacity ? at : -1;
+    weight[team][me] = p.weights ? p.weights[t * p.k + me] : 1.f;
   }
-#pragma unroll
-  for (int i = 0; i < Elem<T>::E; ++i)
-    if (c + i < cols) reinterpret_cast<T*>(row)[c + i] = reinterpret_cast<const T*>(&v)[i];
-}
-
-// A block for a token.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
-  constexpr int E = Elem<T>::E;
-  const long long t = blockIdx.x, row_bytes = p.cols * (long long)sizeof(T);
-  for (long long c = threadIdx.x * E; c < p.cols; c += blockDim.x * E) {
+  if (TEAM > 32) __syncthreads();
+  else __syncwarp();
+  if (t >= p.tokens) return;
+  const int parts = (p.cols + TEAM * E - 1) / (TEAM * E);
+  for (int i = 0; i < parts; ++i) {
     float sum[E], a[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
-    for (int j = 0; j < p.k; ++j) {
-      const long long at = p.positions[t * p.k + j];
-      if (at < 0 || at >= p.capacity) continue;
-      const float w = p.weights ? p.weights[t * p.k + j] : 1.f;
-      Elem<T>::unpack(part<T, VEC>(p.rows + at * row_bytes, c, p.cols), a);
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (p.residual) r = part<T, VEC, TEAM>(p.residual + t * p.residual_stride * (long long)sizeof(T), i, me, p.cols);
+    for (int j = 0; j < p.k; j += AHEAD) {
+      uint4 v[AHEAD];
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum[e] = fmaf(w, a[e], sum[e]);
+      for (int n = 0; n < AHEAD; ++n)
+        if (j + n < p.k && place[team][j + n] >= 0)
+          v[n] = part<T, VEC, TEAM>(p.rows + place[team][j + n] * row_bytes, i, me, p.cols);
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n)
+        if (j + n < p.k && place[team][j + n] >= 0) {
+          const float w = weight[team][j + n];
+          Elem<T>::unpack(v[n], a);
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum[e] = fmaf(w, a[e], sum[e]);
+        }
     }
     if (p.residual) {
-      Elem<T>::unpack(part<T, VEC>(p.residual + t * p.residual_stride * (long long)sizeof(T), c, p.cols), a);
+      Elem<T>::unpack(r, a);
 #pragma unroll
       for (int e = 0; e < E; ++e) sum[e] += a[e];
     }
-    put<T, VEC>(p.out + t * row_bytes, c, p.cols, Elem<T>::pack(sum));
+    put<T, VEC, TEAM>(p.out + t * row_bytes, i, me, p.cols, Elem<T>::pack(sum));
   }
 }
 
@@ -902,50 +956,56 @@ struct CombineGradParams {
   const int* offsets;
   char* grad_rows;
   float* grad_weights;
-  long long tokens, cols, capacity, grad_out_stride;
-  int k, experts;
+  long long slots, capacity, grad_out_stride;
+  int cols, k, experts;
 };
 
+// A warp for a slot: no warp waits for another.  The slots of a token are neighbours, so its
+// row of grad_out comes from memory once and then from the first cache.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) combine_grad_kernel(const __grid_constant__ CombineGradParams p) {
-  constexpr int E = Elem<T>::E;
-  __shared__ float slot[8];
+__global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid_constant__ CombineGradParams p) {
+  constexpr int E = Elem<T>::E, AHEAD = 4;
   const long long row_bytes = p.cols * (long long)sizeof(T);
-  if (blockIdx.x >= p.tokens) {
-    const int e = (int)(blockIdx.x - p.tokens);
-    if (VEC) clear_rows<uint4>(p.grad_rows, p.counts, p.offsets, e, row_bytes, p.capacity);
-    else clear_rows<T>(p.grad_rows, p.counts, p.offsets, e, row_bytes, p.capacity);
+  if (blockIdx.x < p.experts) {
+    if (VEC) clear_rows<uint4>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
+    else clear_rows<T>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
     return;
   }
-  const long long t = blockIdx.x;
-  const char* grad = p.grad_out + t * p.grad_out_stride * (long long)sizeof(T);
-  for (int j = 0; j < p.k; ++j) {
-    const long long at = p.positions[t * p.k + j];
-    float dot = 0.f;
-    if (at >= 0 && at < p.capacity) {
-      const float w = p.weights[t * p.k + j];
-      for (long long c = threadIdx.x * E; c < p.cols; c += blockDim.x * E) {
+  const long long slot = (long long)(blockIdx.x - p.experts) * (kMoveThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (slot >= p.slots) return;
+  const long long at = p.positions[slot];
+  float dot = 0.f;
+  if (at >= 0 && at < p.capacity) {
+    const float w = p.weights[slot];
+    const char* grad = p.grad_out + slot / p.k * p.grad_out_stride * (long long)sizeof(T);
+    const char* row = p.rows + at * row_bytes;
+    char* to = p.grad_rows + at * row_bytes;
+    const int parts = (p.cols + 32 * E - 1) / (32 * E);
+    for (int i = 0; i < parts; i += AHEAD) {
+      uint4 g[AHEAD], y[AHEAD];
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {  // parts behind the last hold zeros and are not written
+        y[n] = part<T, VEC, 32>(row, i + n, lane, p.cols);
+        g[n] = part<T, VEC, 32>(grad, i + n, lane, p.cols);
+      }
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
         float a[E], b[E];
-        Elem<T>::unpack(part<T, VEC>(grad, c, p.cols), a);
-        Elem<T>::unpack(part<T, VEC>(p.rows + at * row_bytes, c, p.cols), b);
+        Elem<T>::unpack(g[n], a);
+        Elem<T>::unpack(y[n], b);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           dot = fmaf(a[e], b[e], dot);
           a[e] *= w;
         }
-        put<T, VEC>(p.grad_rows + at * row_bytes, c, p.cols, Elem<T>::pack(a));
+        put<T, VEC, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
       }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
-    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < (int)blockDim.x >> 5; ++w) dot += slot[w];
-      p.grad_weights[t * p.k + j] = dot;
-    }
-    __syncthreads();
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
+  if (lane == 0) p.grad_weights[slot] = dot;
 }
 
 __global__ void __launch_bounds__(1024) update_bias_kernel(const float* bias, const int* counts, float* out, int experts,
@@ -988,9 +1048,27 @@ const void* route_grad_fn(int experts) {
   if (experts <= 512) return (const void*)route_grad_kernel<T, 32, 16, VEC>;
   return (const void*)route_grad_kernel<T, 32, 32, VEC>;
 }
+// Threads for a token's row of `words` words, of which each thread takes about four.
+int move_team(int64_t words) { return words <= 128 ? 32 : words <= 512 ? 128 : 256; }
+
+// The same for a sum of rows, of which each thread takes one or two parts: what is under way is the rows.
+int combine_team(int64_t parts) { return parts <= 64 ? 32 : parts <= 256 ? 128 : 256; }
+
+template <typename U>
+const void* dispatch_fn(int team) {
+  return team == 32    ? (const void*)dispatch_kernel<U, 32>
+         : team == 128 ? (const void*)dispatch_kernel<U, 128>
+                       : (const void*)dispatch_kernel<U, 256>;
+}
+template <typename T, bool VEC>
+const void* combine_fn(int team) {
+  return team == 32    ? (const void*)combine_kernel<T, VEC, 32>
+         : team == 128 ? (const void*)combine_kernel<T, VEC, 128>
+                       : (const void*)combine_kernel<T, VEC, 256>;
+}
 template <typename T>
-const void* combine_fn(bool vec) {
-  return vec ? (const void*)combine_kernel<T, true> : (const void*)combine_kernel<T, false>;
+const void* combine_fn(bool vec, int team) {
+  return vec ? combine_fn<T, true>(team) : combine_fn<T, false>(team);
 }
 template <typename T>
 const void* combine_grad_fn(bool vec) {
@@ -1012,7 +1090,7 @@ int check_move(int64_t tokens, int k, int64_t capacity, int64_t row) {
   if (tokens < 0 || k < 1 || k > kMaxChoices || tokens * k > INT32_MAX)
     return report_error(DGN_ERR_ARG, "a token has 1..32 choices, a call fewer than 2^31");
   if (capacity < 0 || capacity > INT32_MAX) return report_error(DGN_ERR_ARG, "capacity must be 0..2^31-1 rows");
-  if (row < 1 || row > INT32_MAX) return report_error(DGN_ERR_ARG, "rows must not be empty or pass 2^31-1");
+  if (row < 1 || row > kMaxRow) return report_error(DGN_ERR_ARG, "rows must not be empty or pass 2^30 elements or bytes");
   return DGN_OK;
 }
 
@@ -1176,14 +1254,15 @@ extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_
   p.experts = experts;
   // The widest word that divides the addresses, the strides and the row.
   const auto fits = [&](int w) { return aligned(x, w) && aligned(out, w) && x_stride % w == 0 && row_bytes % w == 0; };
-  const void* fn = fits(16)  ? (const void*)dispatch_kernel<uint4>
-                   : fits(8) ? (const void*)dispatch_kernel<uint2>
-                   : fits(4) ? (const void*)dispatch_kernel<unsigned>
-                   : fits(2) ? (const void*)dispatch_kernel<unsigned short>
-                             : (const void*)dispatch_kernel<unsigned char>;
+  const int word = fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1, team = move_team(row_bytes / word);
+  const void* fn = word == 16  ? dispatch_fn<uint4>(team)
+                   : word == 8 ? dispatch_fn<uint2>(team)
+                   : word == 4 ? dispatch_fn<unsigned>(team)
+                   : word == 2 ? dispatch_fn<unsigned short>(team)
+                               : dispatch_fn<unsigned char>(team);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)(tokens + experts)), dim3(256), 0, stream, args);
+  return launch(fn, dim3((unsigned)(ceil_div(tokens, kMoveThreads / team) + experts)), dim3(kMoveThreads), 0, stream, args);
 }
 
 extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, const float* weights,
@@ -1207,16 +1286,17 @@ extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, co
   p.residual = static_cast<const char*>(residual);
   p.out = static_cast<char*>(out);
   p.tokens = tokens;
-  p.cols = cols;
+  p.cols = (int)cols;
   p.capacity = capacity;
   p.residual_stride = residual_stride;
   p.k = k;
-  const void* fn = dtype == DGN_F32   ? combine_fn<float>(vec)
-                   : dtype == DGN_F16 ? combine_fn<__half>(vec)
-                                      : combine_fn<__nv_bfloat16>(vec);
+  const int team = combine_team(ceil_div(cols, elems));
+  const void* fn = dtype == DGN_F32   ? combine_fn<float>(vec, team)
+                   : dtype == DGN_F16 ? combine_fn<__half>(vec, team)
+                                      : combine_fn<__nv_bfloat16>(vec, team);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)tokens), dim3(256), 0, stream, args);
+  return launch(fn, dim3((unsigned)ceil_div(tokens, kMoveThreads / team)), dim3(kMoveThreads), 0, stream, args);
 }
 
 extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_stride, const void* rows,
@@ -1247,8 +1327,8 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   p.offsets = offsets;
   p.grad_rows = static_cast<char*>(grad_rows);
   p.grad_weights = grad_weights;
-  p.tokens = tokens;
-  p.cols = cols;
+  p.slots = tokens * k;
+  p.cols = (int)cols;
   p.capacity = capacity;
   p.grad_out_stride = grad_out_stride;
   p.k = k;
@@ -1258,7 +1338,7 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
                                       : combine_grad_fn<__nv_bfloat16>(vec);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)(tokens + experts)), dim3(256), 0, stream, args);
+  return launch(fn, dim3((unsigned)(ceil_div(tokens * k, kMoveThreads / 32) + experts)), dim3(kMoveThreads), 0, stream, args);
 }
 
 extern "C" int dgn_expert_update_bias(const float* bias, const int32_t* counts, float* out, int experts, float rate,
