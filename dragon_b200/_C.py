@@ -10,6 +10,8 @@ import os
 _LIB_PATH = os.environ.get("DGN_LIBRARY") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "lib", "libdgn.so")
 
+_TORCH_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "dgn_torch.so")
+
 HANDLE_BYTES = 256
 MAX_RANKS = 8
 
@@ -176,6 +178,28 @@ def lib():
             fn.argtypes = argtypes
         _lib = handle
     return _lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The extension module of the norm and expert operators (csrc/dgn_torch.cc); raises if it has not been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  its libraries first: the module links against them
+        lib()
+        if not os.path.exists(_TORCH_OPS_PATH):
+            raise RuntimeError("{} is missing: build it with `python -m dragon_b200.build` "
+                               "(there is no fallback path)".format(_TORCH_OPS_PATH))
+        loader = importlib.machinery.ExtensionFileLoader("dgn_torch", _TORCH_OPS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("dgn_torch", loader))
+        loader.exec_module(module)
+        _torch_ops = module
+    return _torch_ops
 
 
 def check(status):

@@ -5,16 +5,20 @@
 * ``dragon_b200/lib/libdgn.so``      -- the C-ABI collective library (include/dgn.h)
 * ``dragon_b200/lib/libdragon_collective.so`` -- the C++ operator layer over it
   (built when its sources are present)
+* ``dragon_b200/lib/dgn_torch.so`` -- the torch calls of the norm and expert
+  operators, an extension module (built against the installed torch)
 
 Objects are rebuilt only when a source or header is newer.  nvcc cross-compiles
 without a GPU, so this runs on any machine with the CUDA toolkit.
 """
 
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(ROOT)
@@ -55,6 +59,17 @@ def _headers():
     return hdrs
 
 
+def _torch_object(obj, src):
+    """Command that compiles the extension module's source, and what it depends on."""
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc = os.path.join(torch_dir, "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-c", src, "-o", obj]
+    for path in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), cuda):
+        cmd += ["-isystem", path]
+    return cmd + ["-isystem", sysconfig.get_paths()["include"]], os.path.join(torch_dir, "version.py")
+
+
 def build(verbose=False, extra_flags=()):
     """Build everything that is out of date; returns the path of libdgn.so."""
     nvcc = _nvcc()
@@ -73,6 +88,9 @@ def build(verbose=False, extra_flags=()):
             obj = os.path.join(OBJ, name[:-3] + ".o")
             cmd = [nvcc] + NVCC_FLAGS + list(extra_flags) + ["-c", src, "-o", obj]
             jobs.append((obj, cmd, [src] + hdrs))
+    torch_src, torch_obj = os.path.join(CSRC, "dgn_torch.cc"), os.path.join(OBJ, "dgn_torch.o")
+    torch_cmd, torch_version = _torch_object(torch_obj, torch_src)
+    jobs.append((torch_obj, torch_cmd, [torch_src, torch_version, hdrs[0]]))
     stale = [(o, c) for o, c, deps in jobs if _newer(o, deps)]
     if stale:
         workers = min(len(stale), os.cpu_count() or 4)
@@ -80,7 +98,7 @@ def build(verbose=False, extra_flags=()):
             for out in pool.map(lambda oc: _run(oc[1]), stale):
                 if verbose and out.strip():
                     print(out)
-    objs = [o for o, _, _ in jobs]
+    objs = [o for o, _, _ in jobs if o != torch_obj]
     lib = os.path.join(LIB, "libdgn.so")
     if _newer(lib, objs):
         _run([nvcc] + ARCH + ["-shared", "-o", lib] + objs + ["-Xlinker", "--no-undefined"])
@@ -96,6 +114,12 @@ def build(verbose=False, extra_flags=()):
             _run([nvcc, "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall", "-shared", "-o", op_lib]
                  + srcs + ["-I", os.path.join(REPO, "include"), "-I", op_dir, "-L", LIB, "-ldgn",
                            "-Xlinker", "-rpath", "-Xlinker", "$ORIGIN", "-Xlinker", "--no-undefined"])
+
+    # The extension module; torch's own libraries are loaded by the time it is imported.
+    ext = os.path.join(LIB, "dgn_torch.so")
+    if _newer(ext, [torch_obj, lib]):
+        _run(["g++", "-shared", "-o", ext, torch_obj, "-L", os.path.join(os.path.dirname(torch_version), "lib"), "-ltorch",
+              "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-L", LIB, "-ldgn", "-Wl,-rpath,$ORIGIN"])
     return lib
 
 

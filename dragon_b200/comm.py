@@ -47,10 +47,6 @@ def _stream_ptr(stream, device):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
-# The raw handle of a device's current stream; the public way to it builds a stream object for each call.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _enter_stream(stream, device):
     """Context in which `stream` (a torch stream or a raw handle) is current, so
     that what a call allocates belongs to it."""

@@ -24,7 +24,6 @@ using namespace dgn;
 
 constexpr int kMaxCols = 32768;
 constexpr int kSMs = 148;
-constexpr int kMaxPartials = 8 * kSMs;     // rows of the weight gradient's partial sums: eight blocks on each SM at most
 constexpr float kSmallestAmax = 0x1p-40f;  // groups whose largest value is below this take this one's scale
 constexpr int kThreads = 256;              // of a block whose rows belong to teams of its threads
 
@@ -791,8 +790,15 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
 
 extern "C" int64_t dgn_rms_norm_grad_workspace(int64_t rows, int64_t cols, int dtype) {
   if (!float_dtype(dtype) || rows < 1 || cols < 1 || cols > kMaxCols) return 0;
-  // Enough for either alignment of the rows: a block has one partial sum, and at least one row.
-  return (rows < kMaxPartials ? rows : kMaxPartials) * cols * (int64_t)sizeof(float);
+  // Enough for either alignment of the rows, with a residual's gradient or without: one sum for each block.
+  int64_t most = 0;
+  for (int vec = 0; vec < 2; ++vec)
+    for (int residual = 0; residual < 2; ++residual) {
+      const RowShape s = grad_shape((int)cols, 16 / (int)dgn_dtype_size(dtype), vec);
+      const int64_t blocks = grad_blocks(s, grad_shared(s, vec, residual, cols), rows);
+      most = blocks > most ? blocks : most;
+    }
+  return most * cols * (int64_t)sizeof(float);
 }
 
 extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, const void* grad_hidden,
