@@ -858,36 +858,34 @@ __global__ void __launch_bounds__(kMoveThreads) dispatch_kernel(const __grid_con
   }
 }
 
-// Part i of a row for thread `me` of TEAM: an aligned vector, or E elements TEAM apart so that
-// neighbouring threads still read neighbouring elements.
-template <typename T, bool VEC, int TEAM>
+// Part i (E elements, 16 bytes) of a row for thread `me` of TEAM: words of W neighbouring
+// elements, TEAM words apart, so that neighbouring threads read neighbouring words.  W = E: rows
+// aligned to 16 bytes; W = 2 (16-bit types) and W = 1: other rows.
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef unsigned short type; };
+template <> struct Word<4> { typedef unsigned type; };
+template <> struct Word<16> { typedef uint4 type; };
+
+template <typename T, int W, int TEAM>
 __device__ __forceinline__ uint4 part(const char* row, int i, int me, int cols) {
-  constexpr int E = Elem<T>::E;
+  constexpr int Q = Elem<T>::E / W;
+  typedef typename Word<W * sizeof(T)>::type U;
   uint4 v = make_uint4(0, 0, 0, 0);
-  if (VEC) {
-    const int c = (i * TEAM + me) * E;
-    if (c < cols) v = *reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T));
-  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = (i * E + e) * TEAM + me;
-      if (c < cols) reinterpret_cast<T*>(&v)[e] = reinterpret_cast<const T*>(row)[c];
-    }
+  for (int q = 0; q < Q; ++q) {
+    const int c = ((i * Q + q) * TEAM + me) * W;
+    if (c < cols) reinterpret_cast<U*>(&v)[q] = *reinterpret_cast<const U*>(row + (size_t)c * sizeof(T));
   }
   return v;
 }
-template <typename T, bool VEC, int TEAM>
+template <typename T, int W, int TEAM>
 __device__ __forceinline__ void put(char* row, int i, int me, int cols, uint4 v) {
-  constexpr int E = Elem<T>::E;
-  if (VEC) {
-    const int c = (i * TEAM + me) * E;
-    if (c < cols) *reinterpret_cast<uint4*>(row + (size_t)c * sizeof(T)) = v;
-  } else {
+  constexpr int Q = Elem<T>::E / W;
+  typedef typename Word<W * sizeof(T)>::type U;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = (i * E + e) * TEAM + me;
-      if (c < cols) reinterpret_cast<T*>(row)[c] = reinterpret_cast<const T*>(&v)[e];
-    }
+  for (int q = 0; q < Q; ++q) {
+    const int c = ((i * Q + q) * TEAM + me) * W;
+    if (c < cols) *reinterpret_cast<U*>(row + (size_t)c * sizeof(T)) = reinterpret_cast<const U*>(&v)[q];
   }
 }
 
@@ -903,7 +901,7 @@ struct CombineParams {
 
 // TEAM threads for a token; TWO parts of four of its rows are on their way at a time, and four blocks share an SM:
 // 55.5 us for 8192x2048 bfloat16 with 8 choices, 59.9 with the registers that the compiler would take, 56.6 with one part.
-template <typename T, bool VEC, int TEAM, int TWO>
+template <typename T, int W, int TEAM, int TWO>
 __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_constant__ CombineParams p) {
   constexpr int E = Elem<T>::E, AHEAD = 4;
   __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
@@ -926,7 +924,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
     for (int u = 0; u < TWO; ++u) {
 #pragma unroll
       for (int e = 0; e < E; ++e) sum[u][e] = 0.f;
-      if (p.residual) r[u] = part<T, VEC, TEAM>(p.residual + t * p.residual_stride * (long long)sizeof(T), i + u, me, p.cols);
+      if (p.residual) r[u] = part<T, W, TEAM>(p.residual + t * p.residual_stride * (long long)sizeof(T), i + u, me, p.cols);
     }
     for (int j = 0; j < p.k; j += AHEAD) {
       uint4 v[AHEAD][TWO];
@@ -935,7 +933,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
         if (j + n < p.k && place[team][j + n] >= 0) {
 #pragma unroll
           for (int u = 0; u < TWO; ++u)
-            v[n][u] = part<T, VEC, TEAM>(p.rows + place[team][j + n] * row_bytes, i + u, me, p.cols);
+            v[n][u] = part<T, W, TEAM>(p.rows + place[team][j + n] * row_bytes, i + u, me, p.cols);
         }
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n)
@@ -956,7 +954,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[u][e] += a[e];
       }
-      put<T, VEC, TEAM>(p.out + t * row_bytes, i + u, me, p.cols, Elem<T>::pack(sum[u]));
+      put<T, W, TEAM>(p.out + t * row_bytes, i + u, me, p.cols, Elem<T>::pack(sum[u]));
     }
   }
 }
@@ -976,13 +974,12 @@ struct CombineGradParams {
 
 // A warp for a slot: no warp waits for another.  The slots of a token are neighbours, so its
 // row of grad_out comes from memory once and then from the first cache.
-template <typename T, bool VEC>
+template <typename T, int W>
 __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid_constant__ CombineGradParams p) {
   constexpr int E = Elem<T>::E, AHEAD = 4;
   const long long row_bytes = p.cols * (long long)sizeof(T);
   if (blockIdx.x < p.experts) {
-    if (VEC) clear_rows<uint4>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
-    else clear_rows<T>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
+    clear_rows<typename Word<W * sizeof(T)>::type>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
     return;
   }
   const long long slot = (long long)(blockIdx.x - p.experts) * (kMoveThreads / 32) + (threadIdx.x >> 5);
@@ -1000,8 +997,8 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid
       uint4 g[AHEAD], y[AHEAD];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {  // parts behind the last hold zeros and are not written
-        y[n] = part<T, VEC, 32>(row, i + n, lane, p.cols);
-        g[n] = part<T, VEC, 32>(grad, i + n, lane, p.cols);
+        y[n] = part<T, W, 32>(row, i + n, lane, p.cols);
+        g[n] = part<T, W, 32>(grad, i + n, lane, p.cols);
       }
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
@@ -1013,7 +1010,7 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid
           dot = fmaf(a[e], b[e], dot);
           a[e] *= w;
         }
-        put<T, VEC, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
+        put<T, W, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
       }
     }
   }
@@ -1079,23 +1076,28 @@ const void* dispatch_fn(int team) {
          : team == 128 ? (const void*)dispatch_kernel<U, 128>
                        : (const void*)dispatch_kernel<U, 256>;
 }
-template <typename T, bool VEC>
+template <typename T, int W>
 const void* combine_fn(const CombineTeam& c) {
-  constexpr int TWO = VEC ? 2 : 1;
-  const int team = c.threads;
-  return c.parts == 1  ? (const void*)combine_kernel<T, VEC, 32, 1>
-         : team == 32  ? (const void*)combine_kernel<T, VEC, 32, TWO>
-         : team == 64  ? (const void*)combine_kernel<T, VEC, 64, TWO>
-         : team == 128 ? (const void*)combine_kernel<T, VEC, 128, TWO>
-                       : (const void*)combine_kernel<T, VEC, 256, TWO>;
+  constexpr int TWO = W == Elem<T>::E ? 2 : 1;
+  return c.parts == 1       ? (const void*)combine_kernel<T, W, 32, 1>
+         : c.threads == 32  ? (const void*)combine_kernel<T, W, 32, TWO>
+         : c.threads == 64  ? (const void*)combine_kernel<T, W, 64, TWO>
+         : c.threads == 128 ? (const void*)combine_kernel<T, W, 128, TWO>
+                            : (const void*)combine_kernel<T, W, 256, TWO>;
 }
 template <typename T>
-const void* combine_fn(bool vec, const CombineTeam& team) {
-  return vec ? combine_fn<T, true>(team) : combine_fn<T, false>(team);
+const void* combine_fn(int word, const CombineTeam& team) {
+  if (word == Elem<T>::E) return combine_fn<T, Elem<T>::E>(team);
+  if constexpr (sizeof(T) == 2)
+    if (word == 2) return combine_fn<T, 2>(team);
+  return combine_fn<T, 1>(team);
 }
 template <typename T>
-const void* combine_grad_fn(bool vec) {
-  return vec ? (const void*)combine_grad_kernel<T, true> : (const void*)combine_grad_kernel<T, false>;
+const void* combine_grad_fn(int word) {
+  if (word == Elem<T>::E) return (const void*)combine_grad_kernel<T, Elem<T>::E>;
+  if constexpr (sizeof(T) == 2)
+    if (word == 2) return (const void*)combine_grad_kernel<T, 2>;
+  return (const void*)combine_grad_kernel<T, 1>;
 }
 
 int check_route(int64_t tokens, int64_t stride, int experts, int k, int score, int dtype) {
@@ -1300,8 +1302,12 @@ extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, co
   const int es = (int)dgn_dtype_size(dtype), elems = 16 / es;
   if (!aligned(rows, es) || !aligned(residual, es) || !aligned(out, es) || !aligned(positions, 4) || !aligned(weights, 4))
     return misaligned();
-  const bool vec = cols % elems == 0 && aligned(rows, 16) && aligned(out, 16) &&
-                   (!residual || (aligned(residual, 16) && residual_stride % elems == 0));
+  // Whether words of `w` elements divide the rows and what they lie in.
+  const auto fits = [&](int w) {
+    return cols % w == 0 && aligned(rows, w * es) && aligned(out, w * es) &&
+           (!residual || (aligned(residual, w * es) && residual_stride % w == 0));
+  };
+  const int word = fits(elems) ? elems : es == 2 && fits(2) ? 2 : 1;
   CombineParams p;
   p.rows = static_cast<const char*>(rows);
   p.positions = positions;
@@ -1314,9 +1320,9 @@ extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, co
   p.residual_stride = residual_stride;
   p.k = k;
   const CombineTeam team = combine_team(ceil_div(cols, elems));
-  const void* fn = dtype == DGN_F32   ? combine_fn<float>(vec, team)
-                   : dtype == DGN_F16 ? combine_fn<__half>(vec, team)
-                                      : combine_fn<__nv_bfloat16>(vec, team);
+  const void* fn = dtype == DGN_F32   ? combine_fn<float>(word, team)
+                   : dtype == DGN_F16 ? combine_fn<__half>(word, team)
+                                      : combine_fn<__nv_bfloat16>(word, team);
   DGN_ON(device);
   void* args[] = {&p};
   return launch(fn, dim3((unsigned)ceil_div(tokens, kMoveThreads / team.threads)), dim3(kMoveThreads), 0, stream, args);
@@ -1339,8 +1345,11 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   if (!aligned(grad_out, es) || !aligned(rows, es) || !aligned(grad_rows, es) || !aligned(positions, 4) ||
       !aligned(weights, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(grad_weights, 4))
     return misaligned();
-  const bool vec = cols % elems == 0 && aligned(grad_out, 16) && grad_out_stride % elems == 0 && aligned(rows, 16) &&
-                   aligned(grad_rows, 16);
+  const auto fits = [&](int w) {
+    return cols % w == 0 && grad_out_stride % w == 0 && aligned(grad_out, w * es) && aligned(rows, w * es) &&
+           aligned(grad_rows, w * es);
+  };
+  const int word = fits(elems) ? elems : es == 2 && fits(2) ? 2 : 1;
   CombineGradParams p;
   p.grad_out = static_cast<const char*>(grad_out);
   p.rows = static_cast<const char*>(rows);
@@ -1356,9 +1365,9 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   p.grad_out_stride = grad_out_stride;
   p.k = k;
   p.experts = experts;
-  const void* fn = dtype == DGN_F32   ? combine_grad_fn<float>(vec)
-                   : dtype == DGN_F16 ? combine_grad_fn<__half>(vec)
-                                      : combine_grad_fn<__nv_bfloat16>(vec);
+  const void* fn = dtype == DGN_F32   ? combine_grad_fn<float>(word)
+                   : dtype == DGN_F16 ? combine_grad_fn<__half>(word)
+                                      : combine_grad_fn<__nv_bfloat16>(word);
   DGN_ON(device);
   void* args[] = {&p};
   return launch(fn, dim3((unsigned)(ceil_div(tokens * k, kMoveThreads / 32) + experts)), dim3(kMoveThreads), 0, stream, args);

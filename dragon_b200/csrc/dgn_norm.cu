@@ -42,53 +42,63 @@ struct NormParams {
 };
 
 // Threads and columns.  A row belongs to a team of `team` threads; each of them holds NV
-// parts of E elements (16 bytes).  Aligned rows (VEC): a part is one 16-byte vector, and
-// neighbouring threads have neighbouring vectors.  Other rows: neighbouring threads have
-// neighbouring elements, so that loads of one element each still fill whole lines.
-template <typename T, bool VEC>
+// parts of E elements (16 bytes), made of words of W neighbouring elements.  W = E: rows
+// aligned to 16 bytes.  W = 2 (16-bit types, an even number of columns) and W = 1: other rows.
+// Neighbouring threads have neighbouring words, so that narrow loads still fill whole lines.
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef unsigned short type; };
+template <> struct Word<4> { typedef unsigned type; };
+
+template <typename T, int W>
 __device__ __forceinline__ int column(int i, int e, int thread, int team) {
-  return VEC ? (i * team + thread) * Elem<T>::E + e : (i * Elem<T>::E + e) * team + thread;
+  constexpr int Q = Elem<T>::E / W;
+  return ((i * Q + e / W) * team + thread) * W + e % W;
 }
 
-template <typename T, bool VEC>
+template <typename T, int W>
 __device__ __forceinline__ uint4 load_part(const char* row, int i, int thread, int team, int cols) {
-  if (VEC) {
-    const int c = column<T, VEC>(i, 0, thread, team);
+  constexpr int E = Elem<T>::E;
+  if constexpr (W == E) {
+    const int c = column<T, W>(i, 0, thread, team);
     return c < cols ? *reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T)) : make_uint4(0, 0, 0, 0);
-  }
-  uint4 v = make_uint4(0, 0, 0, 0);
+  } else {
+    typedef typename Word<W * sizeof(T)>::type U;
+    uint4 v = make_uint4(0, 0, 0, 0);
 #pragma unroll
-  for (int e = 0; e < Elem<T>::E; ++e) {
-    const int c = column<T, VEC>(i, e, thread, team);
-    if (c < cols) reinterpret_cast<T*>(&v)[e] = reinterpret_cast<const T*>(row)[c];
+    for (int e = 0; e < E; e += W) {
+      const int c = column<T, W>(i, e, thread, team);
+      if (c < cols) reinterpret_cast<U*>(&v)[e / W] = *reinterpret_cast<const U*>(row + (size_t)c * sizeof(T));
+    }
+    return v;
   }
-  return v;
 }
-template <typename T, bool VEC>
+template <typename T, int W>
 __device__ __forceinline__ void store_part(char* row, int i, int thread, int team, int cols, uint4 v) {
-  if (VEC) {
-    const int c = column<T, VEC>(i, 0, thread, team);
+  constexpr int E = Elem<T>::E;
+  if constexpr (W == E) {
+    const int c = column<T, W>(i, 0, thread, team);
     if (c < cols) *reinterpret_cast<uint4*>(row + (size_t)c * sizeof(T)) = v;
-    return;
-  }
+  } else {
+    typedef typename Word<W * sizeof(T)>::type U;
 #pragma unroll
-  for (int e = 0; e < Elem<T>::E; ++e) {
-    const int c = column<T, VEC>(i, e, thread, team);
-    if (c < cols) reinterpret_cast<T*>(row)[c] = reinterpret_cast<const T*>(&v)[e];
+    for (int e = 0; e < E; e += W) {
+      const int c = column<T, W>(i, e, thread, team);
+      if (c < cols) *reinterpret_cast<U*>(row + (size_t)c * sizeof(T)) = reinterpret_cast<const U*>(&v)[e / W];
+    }
   }
 }
 
 // The weights of a part in float32: ones without a weight, zeros behind the last column.
-template <typename T, bool VEC>
+template <typename T, int W>
 __device__ __forceinline__ void load_weight(const char* weight, int f32, int i, int thread, int team, int cols, float* w) {
   constexpr int E = Elem<T>::E;
   if (!weight) {
 #pragma unroll
     for (int e = 0; e < E; ++e) w[e] = 1.f;
   } else if (!f32) {
-    Elem<T>::unpack(load_part<T, VEC>(weight, i, thread, team, cols), w);
-  } else if (VEC) {
-    const int c = column<T, VEC>(i, 0, thread, team);
+    Elem<T>::unpack(load_part<T, W>(weight, i, thread, team, cols), w);
+  } else if (W == E) {
+    const int c = column<T, W>(i, 0, thread, team);
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
       const float4 f = c < cols ? *reinterpret_cast<const float4*>(weight + (size_t)(c + e) * 4) : make_float4(0, 0, 0, 0);
@@ -96,9 +106,15 @@ __device__ __forceinline__ void load_weight(const char* weight, int f32, int i, 
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = column<T, VEC>(i, e, thread, team);
-      w[e] = c < cols ? reinterpret_cast<const float*>(weight)[c] : 0.f;
+    for (int e = 0; e < E; e += W) {
+      const int c = column<T, W>(i, e, thread, team);
+      const bool there = c < cols;
+      if (W == 2) {
+        const float2 f = there ? *reinterpret_cast<const float2*>(weight + (size_t)c * 4) : make_float2(0, 0);
+        w[e] = f.x; w[e + 1] = f.y;
+      } else {
+        w[e] = there ? *reinterpret_cast<const float*>(weight + (size_t)c * 4) : 0.f;
+      }
     }
   }
 }
@@ -144,10 +160,10 @@ template <typename T> __device__ __forceinline__ uint4 pack2(const Pair* a) {
   }
   return Elem<T>::pack(f);
 }
-template <typename T, bool VEC>
+template <typename T, int W>
 __device__ __forceinline__ void load_weight2(const char* weight, int f32, int i, int thread, int team, int cols, Pair* w) {
   float f[Elem<T>::E];
-  load_weight<T, VEC>(weight, f32, i, thread, team, cols, f);
+  load_weight<T, W>(weight, f32, i, thread, team, cols, f);
 #pragma unroll
   for (int e = 0; e < Elem<T>::E; e += 2) w[e / 2] = Pair(f[e], f[e + 1]);
 }
@@ -231,13 +247,15 @@ __device__ __forceinline__ float code_scale(float m, float rstd, float inv_large
 
 // One row for a block (TEAM 0), or RU rows for a team of TEAM lanes; rows that are read
 // together lie next to each other.
-template <typename T, int TEAM, int NV, bool VEC, bool CODES>
-__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
+template <typename T, int TEAM, int NV, int W, bool CODES>
+__global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThreads : NV == 2 ? 512 : 1024)
     rms_norm_kernel(const __grid_constant__ NormParams p) {
-  constexpr int E = Elem<T>::E, RU = !TEAM || !VEC ? 1 : NV == 1 ? 4 : NV == 2 ? 2 : 1;
+  constexpr int E = Elem<T>::E;
+  constexpr bool VEC = W == E;
+  constexpr int RU = !TEAM || !VEC ? 1 : NV == 1 ? 4 : NV == 2 ? 2 : 1;
   constexpr long long S = sizeof(T);
   __shared__ __align__(16) float slot[2][32];
-  __shared__ unsigned chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
+  __shared__ float chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const long long first = (long long)blockIdx.x * blockDim.y * RU + threadIdx.y;
   uint4 h[RU][NV], r[RU][NV];
@@ -248,8 +266,8 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
     for (int i = 0; i < NV; ++i) {
       h[u][i] = r[u][i] = make_uint4(0, 0, 0, 0);
       if (row < p.rows) {
-        h[u][i] = load_part<T, VEC>(p.x + row * p.x_stride * S, i, me, team, cols);
-        if (p.residual) r[u][i] = load_part<T, VEC>(p.residual + row * p.residual_stride * S, i, me, team, cols);
+        h[u][i] = load_part<T, W>(p.x + row * p.x_stride * S, i, me, team, cols);
+        if (p.residual) r[u][i] = load_part<T, W>(p.residual + row * p.residual_stride * S, i, me, team, cols);
       }
     }
   }
@@ -269,7 +287,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         for (int e = 0; e < E / 2; ++e) a[e] = a[e] + b[e];
         h[u][i] = pack2<T>(a);
         if (sizeof(T) < 4) unpack2<T>(h[u][i], a);
-        if (row < p.rows) store_part<T, VEC>(p.hidden + row * p.hidden_stride * S, i, me, team, cols, h[u][i]);
+        if (row < p.rows) store_part<T, W>(p.hidden + row * p.hidden_stride * S, i, me, team, cols, h[u][i]);
       }
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) squares = fma2(a[e], a[e], squares);
@@ -288,7 +306,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       Pair w[E / 2];
-      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      load_weight2<T, W>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         const long long row = first + u * blockDim.y;
@@ -296,7 +314,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         unpack2<T>(h[u][i], a);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) a[e] = a[e] * twice(rstd[u]) * w[e];
-        if (row < p.rows) store_part<T, VEC>(p.out + row * cols * S, i, me, team, cols, pack2<T>(a));
+        if (row < p.rows) store_part<T, W>(p.out + row * cols * S, i, me, team, cols, pack2<T>(a));
       }
     }
     return;
@@ -313,19 +331,23 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float w[E];
-      load_weight<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      load_weight<T, W>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         float a[E];
         Elem<T>::unpack(h[u][i], a);
+        if (VEC || whole) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float m = a[e] * w[e];
-          top[u] = Largest::of(top[u], m);
-          if (!VEC && !whole) {
-            const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(m)));  // by the bits a NaN is largest
-            const int at = column<T, VEC>(i, e, me, team) >> 5;
-            if ((me & 31) == 0 && at * 32 < cols) chunk[threadIdx.y * 32 + at] = bits;
+          for (int e = 0; e < E; ++e) top[u] = Largest::of(top[u], a[e] * w[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e += W) {  // 32 / W lanes hold a chunk's words
+            float m = fabsf(a[e] * w[e]);
+            if (W == 2) m = Largest::of(m, a[e + 1] * w[e + 1]);
+#pragma unroll
+            for (int d = 16 / W; d; d >>= 1) m = Largest::of(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const int c = column<T, W>(i, e, me, team);
+            if ((c & 31) == 0 && c < cols) chunk[threadIdx.y * 32 + (c >> 5)] = m;
           }
         }
       }
@@ -337,7 +359,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     Pair w[E / 2];
-    load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+    load_weight2<T, W>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
       const long long row = first + u * blockDim.y;
@@ -347,7 +369,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) a[e] = a[e] * w[e];
       if (VEC) {
-        const int c = column<T, VEC>(i, 0, me, team);
+        const int c = column<T, W>(i, 0, me, team);
         float m = 0.f;
         if (whole) {
           m = top[u];
@@ -366,22 +388,27 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         if (E == 8) *reinterpret_cast<uint2*>(out + c) = codes;
         else *reinterpret_cast<unsigned*>(out + c) = codes.x;
       } else {
+        const float all = code_factor(top[u], rstd[u], largest);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int c = column<T, VEC>(i, e, me, team);
+        for (int e = 0; e < E; e += W) {
+          const int c = column<T, W>(i, e, me, team);
           if (c >= cols || row >= p.rows) continue;
-          float m = top[u];
+          float m = top[u], f = all;
           int group = 0;
           if (!whole) {
             group = c >> p.group_shift;
             const int begin = group << (p.group_shift - 5), end = min(begin + (1 << (p.group_shift - 5)), (cols + 31) >> 5);
-            unsigned bits = 0;
-            for (int k = begin; k < end; ++k) bits = max(bits, chunk[threadIdx.y * 32 + k]);
-            m = __uint_as_float(bits);
+            m = 0.f;
+            for (int k = begin; k < end; ++k) m = Largest::of(m, chunk[threadIdx.y * 32 + k]);
+            f = code_factor(m, rstd[u], largest);
           }
           if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = code_scale(m, rstd[u], p.inv_largest);
-          const float v = e & 1 ? a[e / 2].get().y : a[e / 2].get().x;
-          out[c] = (unsigned char)encode1(v * code_factor(m, rstd[u], largest), p.code);
+          const float2 v = a[e / 2].get();
+          if (W == 2)
+            *reinterpret_cast<unsigned short*>(out + c) =
+                (unsigned short)(encode1(v.x * f, p.code) | encode1(v.y * f, p.code) << 8);
+          else
+            out[c] = (unsigned char)encode1((e & 1 ? v.y : v.x) * f, p.code);
         }
       }
     }
@@ -405,9 +432,10 @@ __device__ __forceinline__ float along(float d, float rstd, int cols) { return d
 
 // Writes a block's sums of the weight gradient to its row of the partial sums; teams that
 // share the block are added in shared memory, in their order.
-template <typename T, int TEAM, int NV, bool VEC>
+template <typename T, int TEAM, int NV, int W>
 __device__ __forceinline__ void store_partial(const NormGradParams& p, const Pair* sums, float* shared) {
   constexpr int E = Elem<T>::E;
+  constexpr bool VEC = W == E;
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   float* mine = p.partial + (long long)blockIdx.x * cols;
   float* to = TEAM ? shared + threadIdx.y * cols : mine;
@@ -416,7 +444,7 @@ __device__ __forceinline__ void store_partial(const NormGradParams& p, const Pai
   for (int i = 0; i < NV * E; ++i) acc[i] = i & 1 ? sums[i / 2].get().y : sums[i / 2].get().x;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = column<T, VEC>(i, 0, me, team);
+    const int c = column<T, W>(i, 0, me, team);
     if (VEC && c < cols) {
 #pragma unroll
       for (int e = 0; e < E; e += 4)
@@ -424,7 +452,7 @@ __device__ __forceinline__ void store_partial(const NormGradParams& p, const Pai
     } else if (!VEC) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (column<T, VEC>(i, e, me, team) < cols) to[column<T, VEC>(i, e, me, team)] = acc[i * E + e];
+        if (column<T, W>(i, e, me, team) < cols) to[column<T, W>(i, e, me, team)] = acc[i * E + e];
     }
   }
   if (!TEAM) return;
@@ -438,10 +466,9 @@ __device__ __forceinline__ void store_partial(const NormGradParams& p, const Pai
 
 // The plain form: rows straight into registers.  Taken by rows that are not aligned, by
 // short ones (a team of 8 or 16 lanes, four rows at a time) and by those too long for the ring below.
-template <typename T, int TEAM, int NV, bool VEC>
-__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
-    rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
-  constexpr int E = Elem<T>::E, RU = TEAM && VEC ? 4 : 1;
+template <typename T, int TEAM, int NV, int W, int MOST = TEAM ? kThreads : 512>
+__global__ void __launch_bounds__(MOST, TEAM ? 2 : 1) rms_norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+  constexpr int E = Elem<T>::E, RU = TEAM && W == E ? 4 : 1;
   constexpr long long S = sizeof(T);
   extern __shared__ __align__(16) float shared[];  // teams * cols floats
   __shared__ __align__(16) float slot[2][32];
@@ -462,9 +489,9 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
       for (int i = 0; i < NV; ++i) {
         g[u][i] = h[u][i] = r[u][i] = make_uint4(0, 0, 0, 0);
         if (row < p.rows) {
-          g[u][i] = load_part<T, VEC>(p.grad_out + row * p.grad_out_stride * S, i, me, team, cols);
-          h[u][i] = load_part<T, VEC>(p.hidden + row * p.hidden_stride * S, i, me, team, cols);
-          if (p.grad_hidden) r[u][i] = load_part<T, VEC>(p.grad_hidden + row * p.grad_hidden_stride * S, i, me, team, cols);
+          g[u][i] = load_part<T, W>(p.grad_out + row * p.grad_out_stride * S, i, me, team, cols);
+          h[u][i] = load_part<T, W>(p.hidden + row * p.hidden_stride * S, i, me, team, cols);
+          if (p.grad_hidden) r[u][i] = load_part<T, W>(p.grad_hidden + row * p.grad_hidden_stride * S, i, me, team, cols);
         }
       }
       dot[u] = 0.f;
@@ -472,7 +499,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       Pair w[E / 2];
-      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      load_weight2<T, W>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         Pair a[E / 2], b[E / 2], d(0.f, 0.f);
@@ -490,7 +517,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       Pair w[E / 2];
-      load_weight2<T, VEC>(p.weight, p.weight_f32, i, me, team, cols, w);
+      load_weight2<T, W>(p.weight, p.weight_f32, i, me, team, cols, w);
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         const long long row = base + u * blockDim.y + threadIdx.y;
@@ -501,11 +528,11 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 1024)
         unpack2<T>(r[u][i], c);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) a[e] = fma2(a[e] * w[e], scale, fma2(back, b[e], c[e]));
-        if (row < p.rows) store_part<T, VEC>(p.grad_x + row * cols * S, i, me, team, cols, pack2<T>(a));
+        if (row < p.rows) store_part<T, W>(p.grad_x + row * cols * S, i, me, team, cols, pack2<T>(a));
       }
     }
   }
-  if (p.partial) store_partial<T, TEAM, NV, VEC>(p, acc, shared);
+  if (p.partial) store_partial<T, TEAM, NV, W>(p, acc, shared);
 }
 
 __host__ __device__ constexpr int ring_stages(int vectors) { return vectors == 4 ? 2 : 4; }
@@ -531,7 +558,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
     uint4* to = ring + (size_t)stage * TENSORS * NV * threads + place;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column<T, true>(i, 0, me, team);
+      const int c = column<T, Elem<T>::E>(i, 0, me, team);
       if (row < p.rows && c < cols) {
         copy_async(to + (0 * NV + i) * threads, p.grad_out + (row * p.grad_out_stride + c) * S);
         copy_async(to + (1 * NV + i) * threads, p.hidden + (row * p.hidden_stride + c) * S);
@@ -547,7 +574,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
   Pair w[(KEEP ? NV * E : E) / 2], acc[NV * E / 2];
   if (KEEP) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, w + i * E / 2);
+    for (int i = 0; i < NV; ++i) load_weight2<T, Elem<T>::E>(p.weight, p.weight_f32, i, me, team, cols, w + i * E / 2);
   }
 #pragma unroll
   for (int i = 0; i < NV * E / 2; ++i) acc[i] = twice(0.f);
@@ -565,12 +592,12 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       g[i] = h[i] = make_uint4(0, 0, 0, 0);
-      if (column<T, true>(i, 0, me, team) < cols) {
+      if (column<T, Elem<T>::E>(i, 0, me, team) < cols) {
         g[i] = from[(0 * NV + i) * threads];
         h[i] = from[(1 * NV + i) * threads];
       }
       Pair a[E / 2], b[E / 2], *wi = w + (KEEP ? i * E / 2 : 0), d(0.f, 0.f);
-      if (!KEEP) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
+      if (!KEEP) load_weight2<T, Elem<T>::E>(p.weight, p.weight_f32, i, me, team, cols, wi);
       unpack2<T>(g[i], a);
       unpack2<T>(h[i], b);
 #pragma unroll
@@ -584,10 +611,10 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
     const Pair back = twice(-along(dot[0], rstd, cols)), scale = twice(rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column<T, true>(i, 0, me, team);
+      const int c = column<T, Elem<T>::E>(i, 0, me, team);
       if (c >= cols) continue;
       Pair a[E / 2], b[E / 2], f[E / 2], *wi = w + (KEEP ? i * E / 2 : 0);
-      if (!KEEP) load_weight2<T, true>(p.weight, p.weight_f32, i, me, team, cols, wi);
+      if (!KEEP) load_weight2<T, Elem<T>::E>(p.weight, p.weight_f32, i, me, team, cols, wi);
       unpack2<T>(g[i], a);
       unpack2<T>(h[i], b);
       if (RESIDUAL) unpack2<T>(from[(2 * NV + i) * threads], f);
@@ -600,7 +627,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!p.partial) return;
   if (TEAM) __syncthreads();  // the ring becomes the teams' meeting place
-  store_partial<T, TEAM, NV, true>(p, acc, reinterpret_cast<float*>(ring));
+  store_partial<T, TEAM, NV, Elem<T>::E>(p, acc, reinterpret_cast<float*>(ring));
 }
 
 // Sum of the partial rows: a block of 32 x 32 threads takes 32 columns, a warp every 32nd partial row.
@@ -636,7 +663,7 @@ RowShape row_shape(int cols, int elems, bool vec) {
     const int team = !vec ? 32 : parts <= 8 ? 8 : parts <= 16 ? 16 : 32;
     return {team, parts <= 32 ? 1 : parts <= 64 ? 2 : 4, kThreads / team};
   }
-  const int vectors = parts <= 512 ? 2 : parts <= 4096 ? 4 : 8;
+  const int vectors = parts <= (vec ? 512 : 1024) ? 2 : parts <= 4096 ? 4 : 8;
   return {(int)ceil_div(ceil_div(parts, vectors), 32) * 32, vectors, 1};
 }
 
@@ -649,47 +676,54 @@ RowShape grad_shape(int cols, int elems, bool vec) {
   return {64, 2, 1};
 }
 
-template <typename T, bool VEC, bool CODES>
+template <typename T, int W, bool CODES>
 const void* norm_kernel_of(const RowShape& s) {
-  if constexpr (VEC) {
-    if (s.lanes() == 8) return (const void*)rms_norm_kernel<T, 8, 1, VEC, CODES>;
-    if (s.lanes() == 16) return (const void*)rms_norm_kernel<T, 16, 1, VEC, CODES>;
+  if constexpr (W == Elem<T>::E) {
+    if (s.lanes() == 8) return (const void*)rms_norm_kernel<T, 8, 1, W, CODES>;
+    if (s.lanes() == 16) return (const void*)rms_norm_kernel<T, 16, 1, W, CODES>;
   }
   if (s.lanes() == 32) {
-    if (s.vectors == 1) return (const void*)rms_norm_kernel<T, 32, 1, VEC, CODES>;
-    if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 32, 2, VEC, CODES>;
-    return (const void*)rms_norm_kernel<T, 32, 4, VEC, CODES>;
+    if (s.vectors == 1) return (const void*)rms_norm_kernel<T, 32, 1, W, CODES>;
+    if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 32, 2, W, CODES>;
+    return (const void*)rms_norm_kernel<T, 32, 4, W, CODES>;
   }
-  if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 0, 2, VEC, CODES>;
+  if (s.vectors == 2) return (const void*)rms_norm_kernel<T, 0, 2, W, CODES>;
   if constexpr (Elem<T>::E == 4)  // more than 4096 parts: float32 only
-    if (s.vectors == 8) return (const void*)rms_norm_kernel<T, 0, 8, VEC, CODES>;
-  return (const void*)rms_norm_kernel<T, 0, 4, VEC, CODES>;
+    if (s.vectors == 8) return (const void*)rms_norm_kernel<T, 0, 8, W, CODES>;
+  return (const void*)rms_norm_kernel<T, 0, 4, W, CODES>;
+}
+template <typename T, int W>
+const void* norm_kernel_of(const RowShape& s, bool codes) {
+  return codes ? norm_kernel_of<T, W, true>(s) : norm_kernel_of<T, W, false>(s);
 }
 template <typename T>
-const void* norm_kernel(const RowShape& s, bool vec, bool codes) {
-  if (vec) return codes ? norm_kernel_of<T, true, true>(s) : norm_kernel_of<T, true, false>(s);
-  return codes ? norm_kernel_of<T, false, true>(s) : norm_kernel_of<T, false, false>(s);
+const void* norm_kernel(const RowShape& s, int word, bool codes) {
+  if (word == Elem<T>::E) return norm_kernel_of<T, Elem<T>::E>(s, codes);
+  if constexpr (sizeof(T) == 2)
+    if (word == 2) return norm_kernel_of<T, 2>(s, codes);
+  return norm_kernel_of<T, 1>(s, codes);
 }
 
 // Whether the ring takes a row: aligned, more than 16 parts, and two stages of 512 threads' parts are enough.
 bool ring_takes(const RowShape& s, bool vec) { return vec && s.team > 16 && s.team <= 512; }
 
-template <typename T, bool VEC>
+template <typename T, int W>
 const void* norm_grad_kernel_of(const RowShape& s) {
-  if constexpr (VEC) {
-    if (s.lanes() == 8) return (const void*)rms_norm_grad_kernel<T, 8, 1, VEC>;
-    if (s.lanes() == 16) return (const void*)rms_norm_grad_kernel<T, 16, 1, VEC>;
+  if constexpr (W == Elem<T>::E) {
+    if (s.lanes() == 8) return (const void*)rms_norm_grad_kernel<T, 8, 1, W>;
+    if (s.lanes() == 16) return (const void*)rms_norm_grad_kernel<T, 16, 1, W>;
   } else {
     if (s.lanes() == 32) {
-      if (s.vectors == 1) return (const void*)rms_norm_grad_kernel<T, 32, 1, VEC>;
-      if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 32, 2, VEC>;
-      return (const void*)rms_norm_grad_kernel<T, 32, 4, VEC>;
+      if (s.vectors == 1) return (const void*)rms_norm_grad_kernel<T, 32, 1, W>;
+      if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 32, 2, W>;
+      return (const void*)rms_norm_grad_kernel<T, 32, 4, W>;
     }
-    if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 0, 2, VEC>;
+    if (s.vectors == 2) return (const void*)rms_norm_grad_kernel<T, 0, 2, W>;
+    if (s.team <= 512) return (const void*)rms_norm_grad_kernel<T, 0, 4, W>;
   }
   if constexpr (Elem<T>::E == 4)
-    if (s.vectors == 8) return (const void*)rms_norm_grad_kernel<T, 0, 8, VEC>;
-  return (const void*)rms_norm_grad_kernel<T, 0, 4, VEC>;
+    if (s.vectors == 8) return (const void*)rms_norm_grad_kernel<T, 0, 8, W, 1024>;
+  return (const void*)rms_norm_grad_kernel<T, 0, 4, W, 1024>;
 }
 template <typename T, bool RESIDUAL>
 const void* norm_grad_ring_of(const RowShape& s) {
@@ -700,9 +734,13 @@ const void* norm_grad_ring_of(const RowShape& s) {
   return (const void*)rms_norm_grad_ring_kernel<T, 0, 4, RESIDUAL>;
 }
 template <typename T>
-const void* norm_grad_kernel(const RowShape& s, bool vec, bool residual) {
-  if (ring_takes(s, vec)) return residual ? norm_grad_ring_of<T, true>(s) : norm_grad_ring_of<T, false>(s);
-  return vec ? norm_grad_kernel_of<T, true>(s) : norm_grad_kernel_of<T, false>(s);
+const void* norm_grad_kernel(const RowShape& s, int word, bool residual) {
+  constexpr int E = Elem<T>::E;
+  if (ring_takes(s, word == E)) return residual ? norm_grad_ring_of<T, true>(s) : norm_grad_ring_of<T, false>(s);
+  if (word == E) return norm_grad_kernel_of<T, E>(s);
+  if constexpr (sizeof(T) == 2)
+    if (word == 2) return norm_grad_kernel_of<T, 2>(s);
+  return norm_grad_kernel_of<T, 1>(s);
 }
 
 // Shared memory of a backward block.
@@ -751,10 +789,15 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
   if (!aligned(x, es) || !aligned(residual, es) || !aligned(hidden, es) || !aligned(out, code ? 1 : es) ||
       (weight && !aligned(weight, ws)) || !aligned(scales, 4) || !aligned(rstd, 4))
     return report_error(DGN_ERR_ARG, "a pointer is not aligned to its element size");
-  const bool vec = cols % elems == 0 && aligned(x, 16) && x_stride % elems == 0 && aligned(out, 16) &&
-                   (!weight || aligned(weight, 16)) &&
-                   (!residual || (aligned(residual, 16) && aligned(hidden, 16) && residual_stride % elems == 0 &&
-                                  hidden_stride % elems == 0));
+  // Whether words of `w` elements divide the rows and what they lie in.
+  const auto fits = [&](int w) {
+    const size_t bytes = (size_t)w * es;
+    return cols % w == 0 && x_stride % w == 0 && aligned(x, bytes) && aligned(out, code ? w : bytes) &&
+           (!weight || aligned(weight, w * ws > 16 ? 16 : w * ws)) &&
+           (!residual || (residual_stride % w == 0 && hidden_stride % w == 0 && aligned(residual, bytes) && aligned(hidden, bytes)));
+  };
+  const int word = fits(elems) ? elems : es == 2 && fits(2) ? 2 : 1;
+  const bool vec = word == elems;
   const RowShape s = row_shape((int)cols, elems, vec);
   NormParams p;
   p.x = static_cast<const char*>(x);
@@ -777,9 +820,9 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
   p.inv_cols = 1.f / (float)cols;
   p.largest = code == DGN_CODE_I8 ? 127.f : code == DGN_CODE_E4M3 ? 448.f : 57344.f;
   p.inv_largest = 1.f / p.largest;
-  const void* fn = dtype == DGN_F32   ? norm_kernel<float>(s, vec, code != 0)
-                   : dtype == DGN_F16 ? norm_kernel<__half>(s, vec, code != 0)
-                                      : norm_kernel<__nv_bfloat16>(s, vec, code != 0);
+  const void* fn = dtype == DGN_F32   ? norm_kernel<float>(s, word, code != 0)
+                   : dtype == DGN_F16 ? norm_kernel<__half>(s, word, code != 0)
+                                      : norm_kernel<__nv_bfloat16>(s, word, code != 0);
   OnDevice on(device);
   if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()));
   // Rows of a block, as in the kernel: short aligned rows are taken four (one part) or two (two parts) at a time.
@@ -829,10 +872,15 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   if (!aligned(grad_out, es) || !aligned(hidden, es) || !aligned(grad_hidden, es) || !aligned(grad_x, es) ||
       (weight && !aligned(weight, ws)) || !aligned(rstd, 4) || !aligned(workspace, 4))
     return report_error(DGN_ERR_ARG, "a pointer is not aligned to its element size");
-  const bool vec = cols % elems == 0 && aligned(grad_out, 16) && grad_out_stride % elems == 0 && aligned(hidden, 16) &&
-                   hidden_stride % elems == 0 && aligned(grad_x, 16) && (!weight || aligned(weight, 16)) &&
-                   (!grad_hidden || (aligned(grad_hidden, 16) && grad_hidden_stride % elems == 0)) &&
-                   aligned(workspace, 16);
+  const auto fits = [&](int w) {
+    const size_t bytes = (size_t)w * es;
+    return cols % w == 0 && grad_out_stride % w == 0 && hidden_stride % w == 0 && aligned(grad_out, bytes) &&
+           aligned(hidden, bytes) && aligned(grad_x, bytes) && (!weight || aligned(weight, w * ws > 16 ? 16 : w * ws)) &&
+           (w == 1 || aligned(workspace, 16)) &&
+           (!grad_hidden || (grad_hidden_stride % w == 0 && aligned(grad_hidden, bytes)));
+  };
+  const int word = fits(elems) ? elems : es == 2 && fits(2) ? 2 : 1;
+  const bool vec = word == elems;
   const RowShape s = grad_shape((int)cols, elems, vec);
   const size_t smem = grad_shared(s, vec, grad_hidden != nullptr, cols);
   const int parts = grad_blocks(s, smem, rows);
@@ -853,9 +901,9 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   p.cols = (int)cols;
   p.weight_f32 = weight_dtype == DGN_F32;
   const bool residual = grad_hidden != nullptr;
-  const void* fn = dtype == DGN_F32   ? norm_grad_kernel<float>(s, vec, residual)
-                   : dtype == DGN_F16 ? norm_grad_kernel<__half>(s, vec, residual)
-                                      : norm_grad_kernel<__nv_bfloat16>(s, vec, residual);
+  const void* fn = dtype == DGN_F32   ? norm_grad_kernel<float>(s, word, residual)
+                   : dtype == DGN_F16 ? norm_grad_kernel<__half>(s, word, residual)
+                                      : norm_grad_kernel<__nv_bfloat16>(s, word, residual);
   void* args[] = {&p};
   rc = launch(fn, dim3(parts), dim3(s.team, s.teams), smem, stream, args);
   if (rc != DGN_OK || !grad_weight) return rc;

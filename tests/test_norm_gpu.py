@@ -76,7 +76,8 @@ def test_forward(dgn_lib, rows, cols, dtype, kind):
     assert r.scale is None
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 769), (5, 128), (4, 4096), (2, 32768), (9, 200), (130, 96), (3, 2056)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 769), (5, 128), (4, 4096), (2, 32768), (9, 200), (130, 96), (3, 2056), (3, 1030),
+                                       (5, 70), (2, 4228)])
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("out_dtype", list(CODES))
 @pytest.mark.parametrize("group", [0, 32, 64, 128])
