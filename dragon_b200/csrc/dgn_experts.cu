@@ -504,9 +504,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     need = 5 + (unsigned)fminf((slack + 0x1p-22f * fmaxf(fabsf(most), fabsf(base))) * scale, 1e6f);
   }
   unsigned last = kWrap;
-  const bool certain = sizeof(T) == 2 && !p.bias;
-  const int wanted = p.k + (certain ? 0 : 2);
-  for (int j = 0; j < wanted; ++j) {
+  const auto next_word = [&](int j) {
     unsigned best = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) best = __viaddmax_u32(word[i], -last, best);
@@ -514,7 +512,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     last = team_max<L>(best);
     if (lane == j % L) win[j] = last;
     if (last == 0) last = 1;  // nothing is left: only zeros stay below
-  }
+  };
+  const bool certain = sizeof(T) == 2 && !p.bias;
+  const int wanted = p.k + (certain ? 0 : 1);
+  for (int j = 0; j < wanted; ++j) next_word(j);
   __syncwarp();
   if (!certain) {
     bool near = false;
@@ -528,6 +529,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     const unsigned team_lanes = L == 32 ? ~0u : ((1u << (L & 31)) - 1) << (team * L);
     const unsigned all = __ballot_sync(kFull, near && live);
     if (all) {
+      next_word(p.k + 1);  // those that are left over stay below this one
+      __syncwarp();
       near = all & team_lanes;
       if (near && win[p.k + 1]) odd |= (win[p.k - 1] >> p.bits) - (win[p.k + 1] >> p.bits) < need;
       sort_exact<T, L>(p, row, near, win, exact_key, low);
@@ -585,7 +588,7 @@ struct RouteGradParams {
 template <typename T, int L, int N, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
   constexpr int Q = kMaxChoices / L, V = VEC ? 16 / (int)sizeof(T) : 1;
-  __shared__ float direct[kRouteThreads / L][N * L];
+  __shared__ __align__(16) float direct[kRouteThreads / L][N * L];
   __shared__ int chosen[kRouteThreads / L][kMaxChoices];
   __shared__ float slope[kRouteThreads / L][kMaxChoices];
   const int lane = threadIdx.x % L, team = threadIdx.x / L, experts = p.experts;
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_
     logit[q] = index[q] < 0 ? -INFINITY : widen(row[index[q]]);
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) direct[team][i * L + lane] = 0.f;
+  for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(&direct[team][i * L + lane * 4]) = make_float4(0, 0, 0, 0);
   float top = 0.f, inv = 1.f;
   if (!p.sigmoid) {
     top = -INFINITY;
@@ -711,6 +714,7 @@ struct PlanParams {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int hist[];
+  allow_next();
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   const long long first = blockIdx.x * p.span, last = min(first + p.span, p.slots);
@@ -737,6 +741,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
     if (e >= 0 && e < experts) atomicAdd(&hist[warp * experts + e], 1);
   }
   __syncthreads();
+  if (gridDim.x > 1) await_previous();  // the slots have been counted meanwhile
   // Block starts: a scan of the aligned totals over the experts, two experts for a thread.
   int total[2] = {0, 0}, before[2] = {0, 0}, blocks[2];
 #pragma unroll
@@ -1252,7 +1257,8 @@ extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int expert
     if (rc != DGN_OK) return rc;
   }
   const int smem = kPlanWarps * experts * (int)sizeof(int);
-  return launch((const void*)plan_place_kernel, dim3(blocks), dim3(kPlanThreads), smem, stream, args);
+  const auto put_in = blocks > 1 ? launch_behind : launch;
+  return put_in((const void*)plan_place_kernel, dim3(blocks), dim3(kPlanThreads), smem, stream, args);
 }
 
 extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_bytes, const int32_t* positions,

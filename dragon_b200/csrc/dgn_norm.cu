@@ -472,6 +472,7 @@ __global__ void __launch_bounds__(MOST, TEAM ? 2 : 1) rms_norm_grad_kernel(const
   constexpr long long S = sizeof(T);
   extern __shared__ __align__(16) float shared[];  // teams * cols floats
   __shared__ __align__(16) float slot[2][32];
+  allow_next();
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   Pair acc[NV * E / 2];
 #pragma unroll
@@ -535,6 +536,7 @@ __global__ void __launch_bounds__(MOST, TEAM ? 2 : 1) rms_norm_grad_kernel(const
   if (p.partial) store_partial<T, TEAM, NV, W>(p, acc, shared);
 }
 
+// Stages of a ring: four, or two where a thread has four parts.
 __host__ __device__ constexpr int ring_stages(int vectors) { return vectors == 4 ? 2 : 4; }
 
 __device__ __forceinline__ void copy_async(uint4* to, const char* from) {
@@ -545,12 +547,13 @@ __device__ __forceinline__ void copy_async(uint4* to, const char* from) {
 // (cp.async), so the loads of STAGES - 1 rows are in flight while one is worked on and nobody waits for another
 // thread's copy; the sums of the weight gradient (and up to 16 weights a thread) stay in
 // registers for all of the block's rows.
-template <typename T, int TEAM, int NV, bool RESIDUAL>
-__global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
+template <typename T, int TEAM, int NV, bool RESIDUAL, int MOST = NV == 4 ? 512 : kThreads>
+__global__ void __launch_bounds__(MOST) rms_norm_grad_ring_kernel(const __grid_constant__ NormGradParams p) {
   constexpr int E = Elem<T>::E, STAGES = ring_stages(NV), TENSORS = RESIDUAL ? 3 : 2;
   constexpr long long S = sizeof(T);
   extern __shared__ __align__(16) uint4 ring[];  // [STAGES][TENSORS][NV][threads]
   __shared__ __align__(16) float slot[2][32];
+  allow_next();
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const int threads = blockDim.x * blockDim.y, place = threadIdx.y * blockDim.x + me;
   const long long step = (long long)gridDim.x * blockDim.y;
@@ -570,7 +573,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
   long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) fetch(s, row + s * step);
-  constexpr bool KEEP = NV * E <= 16;  // the weights in registers; more of them are read again for each row
+  constexpr bool KEEP = NV <= 2;  // the weights in registers; those of four parts are read again for each row
   Pair w[(KEEP ? NV * E : E) / 2], acc[NV * E / 2];
   if (KEEP) {
 #pragma unroll
@@ -634,6 +637,7 @@ __global__ void __launch_bounds__(TEAM || NV == 2 ? kThreads : 512) rms_norm_gra
 template <typename W>
 __global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* partial, W* grad, int parts, int cols) {
   __shared__ float s[32][33];
+  await_previous();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.f;
   if (c < cols) {
@@ -667,13 +671,13 @@ RowShape row_shape(int cols, int elems, bool vec) {
   return {(int)ceil_div(ceil_div(parts, vectors), 32) * 32, vectors, 1};
 }
 
-// The backward pass keeps the weights and their gradient in registers: two parts a thread wherever that will do, and so
-// a block already for rows of more than 64 parts (1024 columns of bfloat16, 32768 rows: 55.7 us with four parts in a
-// warp, which reads the weights again for each row).
+// The backward pass keeps the weights and their gradient in registers: two parts a thread wherever 512 threads will do.
+// With four, whose weights are read again for each row, 32768 rows of 1024 bfloat16 columns took 55.7 us instead of 47.9;
+// two for each of 1024 threads spill (2048 rows of 16384 columns: 85 us, 78 with four for 512).
 RowShape grad_shape(int cols, int elems, bool vec) {
   const int parts = (int)ceil_div(cols, elems);
-  if (!vec || parts <= 64 || parts > 128) return row_shape(cols, elems, vec);
-  return {64, 2, 1};
+  if (!vec || parts <= 64 || parts > 1024) return row_shape(cols, elems, vec);
+  return {(int)ceil_div(parts, 64) * 32, 2, 1};
 }
 
 template <typename T, int W, bool CODES>
@@ -730,8 +734,9 @@ const void* norm_grad_ring_of(const RowShape& s) {
   if (s.lanes() == 32)
     return s.vectors == 1 ? (const void*)rms_norm_grad_ring_kernel<T, 32, 1, RESIDUAL>
                           : (const void*)rms_norm_grad_ring_kernel<T, 32, 2, RESIDUAL>;
-  if (s.vectors == 2) return (const void*)rms_norm_grad_ring_kernel<T, 0, 2, RESIDUAL>;
-  return (const void*)rms_norm_grad_ring_kernel<T, 0, 4, RESIDUAL>;
+  if (s.vectors == 4) return (const void*)rms_norm_grad_ring_kernel<T, 0, 4, RESIDUAL>;
+  return s.team <= kThreads ? (const void*)rms_norm_grad_ring_kernel<T, 0, 2, RESIDUAL>
+                            : (const void*)rms_norm_grad_ring_kernel<T, 0, 2, RESIDUAL, 512>;
 }
 template <typename T>
 const void* norm_grad_kernel(const RowShape& s, int word, bool residual) {
@@ -913,5 +918,5 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   const void* fn2 = weight_dtype == DGN_F32 ? (const void*)norm_weight_grad_kernel<float>
                     : dtype == DGN_F16      ? (const void*)norm_weight_grad_kernel<__half>
                                             : (const void*)norm_weight_grad_kernel<__nv_bfloat16>;
-  return launch(fn2, dim3((unsigned)ceil_div(cols, 32)), dim3(32, 32), 0, stream, args2);
+  return launch_behind(fn2, dim3((unsigned)ceil_div(cols, 32)), dim3(32, 32), 0, stream, args2);
 }

@@ -58,6 +58,38 @@ inline int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* stre
   return DGN_OK;
 }
 
+// The same for a kernel that reads what the launch before it on the stream has written: its
+// blocks may be placed while the other's finish, and wait there (await_previous) for them all.
+// Saves the gap between two short kernels.
+inline int launch_behind(const void* fn, dim3 grid, dim3 block, size_t smem, void* stream, void** args) {
+  int rc = allow_shared(fn, smem);
+  if (rc != DGN_OK) return rc;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelExC(&config, fn, args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
+  }
+  count_launch();
+  return DGN_OK;
+}
+
+#ifdef __CUDACC__
+// First statement of the kernel in front: the one behind may be placed.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+// First statement of the kernel behind: all blocks of the one in front have ended and what they wrote is there.
+__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool float_dtype(int dtype) { return dtype == DGN_F16 || dtype == DGN_BF16 || dtype == DGN_F32; }
