@@ -333,7 +333,7 @@ __host__ __device__ inline int route_shared(int experts, int groups, int teams) 
 // they are too near the border, or a value is not finite, route_exact makes the whole choice.  16-bit
 // logits without a bias lose nothing with the lowest bits and need none of this.
 template <typename T, int L, int N, bool VEC>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(const __grid_constant__ RouteParams p) {
   constexpr int TEAMS = 32 / L;
   constexpr unsigned kWrap = 1u << 31;
   extern __shared__ __align__(16) char shared[];
@@ -728,10 +728,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const __grid_c
 
 // Every block adds up the counts of the blocks before it, then ranks its own slots: warp w takes the w-th run of them.
 __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_constant__ PlanParams p) {
-  extern __shared__ int hist[];  // [kPlanWarps][experts], then the place of each warp's next slot of an expert
+  extern __shared__ int hist[];  // [kPlanWarps][experts], then the place of each warp's next slot of an expert; [2][experts]
   __shared__ int carry[kPlanWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, experts = p.experts;
-  for (int i = threadIdx.x; i < kPlanWarps * experts; i += blockDim.x) hist[i] = 0;
+  for (int i = threadIdx.x; i < (kPlanWarps + 2) * experts; i += blockDim.x) hist[i] = 0;
   __syncthreads();
   const long long first = blockIdx.x * p.span, last = min(first + p.span, p.slots);
   const long long run = (p.span / 32 + kPlanWarps - 1) / kPlanWarps * 32;
@@ -740,8 +740,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
     const int e = p.indices[s];
     if (e >= 0 && e < experts) atomicAdd(&hist[warp * experts + e], 1);
   }
+  if (gridDim.x > 1) {
+    await_previous();  // the slots have been counted meanwhile
+    int* sums = hist + kPlanWarps * experts;  // [2][experts]: of all blocks, and of those before this one
+    for (int b = warp; b < (int)gridDim.x; b += kPlanWarps)
+      for (int e = lane; e < experts; e += 32) {
+        const int n = p.parts[(long long)b * experts + e];
+        if (!n) continue;
+        atomicAdd(&sums[e], n);
+        if (b < (int)blockIdx.x) atomicAdd(&sums[experts + e], n);
+      }
+  }
   __syncthreads();
-  if (gridDim.x > 1) await_previous();  // the slots have been counted meanwhile
   // Block starts: a scan of the aligned totals over the experts, two experts for a thread.
   int total[2] = {0, 0}, before[2] = {0, 0}, blocks[2];
 #pragma unroll
@@ -751,11 +761,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
       if (gridDim.x == 1) {
         for (int w = 0; w < kPlanWarps; ++w) total[i] += hist[w * experts + e];
       } else {
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-          const int n = p.parts[(long long)b * experts + e];
-          if (b < (int)blockIdx.x) before[i] += n;
-          total[i] += n;
-        }
+        total[i] = hist[kPlanWarps * experts + e];
+        before[i] = hist[(kPlanWarps + 1) * experts + e];
       }
     }
     blocks[i] = (total[i] + p.align - 1) / p.align * p.align;
@@ -1256,7 +1263,7 @@ extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int expert
     rc = launch((const void*)plan_count_kernel, dim3(blocks), dim3(kPlanThreads), experts * sizeof(int), stream, args);
     if (rc != DGN_OK) return rc;
   }
-  const int smem = kPlanWarps * experts * (int)sizeof(int);
+  const int smem = (kPlanWarps + 2) * experts * (int)sizeof(int);
   const auto put_in = blocks > 1 ? launch_behind : launch;
   return put_in((const void*)plan_place_kernel, dim3(blocks), dim3(kPlanThreads), smem, stream, args);
 }
