@@ -136,7 +136,7 @@ SIGNATURES.update({
     "dgn_route": _signature("plpppp" "liiiiiii" "f" "iip"),
     "dgn_route_grad": _signature("pplpp" "liiii" "f" "iip"),
     "dgn_expert_plan_workspace": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int]),
-    "dgn_expert_plan": _signature("pliippppl" "ip"),
+    "dgn_expert_plan": _signature("pliipppppl" "ip"),
     "dgn_expert_dispatch": _signature("pllpppp" "liil" "ip"),
     "dgn_expert_combine": _signature("ppppl" "plill" "iip"),
     "dgn_expert_combine_grad": _signature("plpppppp" "pliill" "iip"),

@@ -52,6 +52,8 @@ def _enter_stream(stream, device):
     that what a call allocates belongs to it."""
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=device)
+    if stream.device != device:
+        raise ValueError("the stream must be one of {} (got {})".format(device, stream.device))
     return torch.cuda.stream(stream)
 
 

@@ -706,6 +706,7 @@ struct PlanParams {
   const int* indices;
   int* counts;
   int* offsets;
+  int* ends;
   int* positions;
   int* parts;  // [gridDim.x][experts]: how often each block's slots ask for each expert
   long long slots, span;  // span: slots of a block, a multiple of 32
@@ -784,6 +785,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const __grid_c
       if (blockIdx.x == 0) {
         p.counts[e] = total[i];
         p.offsets[e] = start;
+        p.ends[e] = start + total[i];
         if (e == experts - 1) p.offsets[experts] = start + blocks[i];
       }
       int next = start + before[i];
@@ -817,8 +819,8 @@ constexpr int kMoveThreads = 256;
 struct MoveParams {
   const char* x;
   const int* positions;
-  const int* counts;
   const int* offsets;
+  const int* ends;
   char* out;
   long long tokens, x_stride, row_bytes, capacity;  // bytes
   int k, experts;
@@ -827,9 +829,9 @@ struct MoveParams {
 // Zeros in the rows of an expert's block that no slot uses, by a whole block of threads.
 // Such blocks come first in the grid: behind the others they would be its tail.
 template <typename U>
-__device__ void clear_rows(char* out, const int* counts, const int* offsets, int e, long long row_bytes,
+__device__ void clear_rows(char* out, const int* offsets, const int* ends, int e, long long row_bytes,
                            long long capacity) {
-  const long long first = max(0ll, (long long)offsets[e] + counts[e]), last = min((long long)offsets[e + 1], capacity);
+  const long long first = max(0, ends[e]), last = min((long long)offsets[e + 1], capacity);
   if (first >= last) return;
   U* to = reinterpret_cast<U*>(out + first * row_bytes);
   const long long n = (last - first) * row_bytes / (long long)sizeof(U);
@@ -842,7 +844,7 @@ __device__ void clear_rows(char* out, const int* counts, const int* offsets, int
 template <typename U, int TEAM>
 __global__ void __launch_bounds__(kMoveThreads) dispatch_kernel(const __grid_constant__ MoveParams p) {
   if (blockIdx.x < p.experts) {
-    clear_rows<U>(p.out, p.counts, p.offsets, blockIdx.x, p.row_bytes, p.capacity);
+    clear_rows<U>(p.out, p.offsets, p.ends, blockIdx.x, p.row_bytes, p.capacity);
     return;
   }
   __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
@@ -976,8 +978,8 @@ struct CombineGradParams {
   const char* rows;
   const int* positions;
   const float* weights;
-  const int* counts;
   const int* offsets;
+  const int* ends;
   char* grad_rows;
   float* grad_weights;
   long long slots, capacity, grad_out_stride;
@@ -991,7 +993,7 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid
   constexpr int E = Elem<T>::E, AHEAD = 4;
   const long long row_bytes = p.cols * (long long)sizeof(T);
   if (blockIdx.x < p.experts) {
-    clear_rows<typename Word<W * sizeof(T)>::type>(p.grad_rows, p.counts, p.offsets, blockIdx.x, row_bytes, p.capacity);
+    clear_rows<typename Word<W * sizeof(T)>::type>(p.grad_rows, p.offsets, p.ends, blockIdx.x, row_bytes, p.capacity);
     return;
   }
   const long long slot = (long long)(blockIdx.x - p.experts) * (kMoveThreads / 32) + (threadIdx.x >> 5);
@@ -1232,16 +1234,16 @@ extern "C" int64_t dgn_expert_plan_workspace(int64_t slots, int experts) {
 }
 
 extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int experts, int align, int32_t* counts,
-                               int32_t* offsets, int32_t* positions, void* workspace, int64_t workspace_bytes,
-                               int device, void* stream) {
+                               int32_t* offsets, int32_t* ends, int32_t* positions, void* workspace,
+                               int64_t workspace_bytes, int device, void* stream) {
   int rc = check_experts(experts);
   if (rc != DGN_OK) return rc;
   if (slots < 0 || slots > INT32_MAX) return report_error(DGN_ERR_ARG, "a call takes 0..2^31-1 slots");
   if (align < 1 || slots + (slots < experts ? slots : experts) * ((int64_t)align - 1) > INT32_MAX)
     return report_error(DGN_ERR_ARG, "align must be positive and the rows fewer than 2^31");
-  if (!counts || !offsets || (slots && (!indices || !positions))) return null_pointer("dgn_expert_plan: null pointer");
-  if (!aligned(indices, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(positions, 4) ||
-      !aligned(workspace, 4))
+  if (!counts || !offsets || !ends || (slots && (!indices || !positions))) return null_pointer("dgn_expert_plan: null pointer");
+  if (!aligned(indices, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(ends, 4) ||
+      !aligned(positions, 4) || !aligned(workspace, 4))
     return misaligned();
   const int64_t need = dgn_expert_plan_workspace(slots, experts);
   if (need && (!workspace || workspace_bytes < need))
@@ -1250,6 +1252,7 @@ extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int expert
   p.indices = indices;
   p.counts = counts;
   p.offsets = offsets;
+  p.ends = ends;
   p.positions = positions;
   p.parts = static_cast<int*>(workspace);
   p.slots = slots;
@@ -1269,20 +1272,20 @@ extern "C" int dgn_expert_plan(const int32_t* indices, int64_t slots, int expert
 }
 
 extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_bytes, const int32_t* positions,
-                                   const int32_t* counts, const int32_t* offsets, void* out, int64_t tokens, int k,
+                                   const int32_t* offsets, const int32_t* ends, void* out, int64_t tokens, int k,
                                    int experts, int64_t capacity, int device, void* stream) {
   int rc = check_move(tokens, k, capacity, row_bytes);
   if (rc == DGN_OK) rc = check_experts(experts);
   if (rc != DGN_OK) return rc;
   if (x_stride < row_bytes) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
   if (tokens == 0 || capacity == 0) return DGN_OK;
-  if (!x || !positions || !counts || !offsets || !out) return null_pointer("dgn_expert_dispatch: null pointer");
-  if (!aligned(positions, 4) || !aligned(counts, 4) || !aligned(offsets, 4)) return misaligned();
+  if (!x || !positions || !offsets || !ends || !out) return null_pointer("dgn_expert_dispatch: null pointer");
+  if (!aligned(positions, 4) || !aligned(offsets, 4) || !aligned(ends, 4)) return misaligned();
   MoveParams p;
   p.x = static_cast<const char*>(x);
   p.positions = positions;
-  p.counts = counts;
   p.offsets = offsets;
+  p.ends = ends;
   p.out = static_cast<char*>(out);
   p.tokens = tokens;
   p.x_stride = x_stride;
@@ -1342,8 +1345,8 @@ extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, co
 }
 
 extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_stride, const void* rows,
-                                       const int32_t* positions, const float* weights, const int32_t* counts,
-                                       const int32_t* offsets, void* grad_rows, float* grad_weights, int64_t tokens,
+                                       const int32_t* positions, const float* weights, const int32_t* offsets,
+                                       const int32_t* ends, void* grad_rows, float* grad_weights, int64_t tokens,
                                        int k, int experts, int64_t cols, int64_t capacity, int dtype, int device,
                                        void* stream) {
   int rc = check_move(tokens, k, capacity, cols);
@@ -1352,11 +1355,11 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   if (!float_dtype(dtype)) return report_error(DGN_ERR_UNSUPPORTED, "rows are float16, bfloat16 or float32");
   if (grad_out_stride < cols) return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
   if (tokens == 0) return DGN_OK;
-  if (!grad_out || !positions || !weights || !counts || !offsets || !grad_weights || (capacity && (!rows || !grad_rows)))
+  if (!grad_out || !positions || !weights || !offsets || !ends || !grad_weights || (capacity && (!rows || !grad_rows)))
     return null_pointer("dgn_expert_combine_grad: null pointer");
   const int es = (int)dgn_dtype_size(dtype), elems = 16 / es;
   if (!aligned(grad_out, es) || !aligned(rows, es) || !aligned(grad_rows, es) || !aligned(positions, 4) ||
-      !aligned(weights, 4) || !aligned(counts, 4) || !aligned(offsets, 4) || !aligned(grad_weights, 4))
+      !aligned(weights, 4) || !aligned(offsets, 4) || !aligned(ends, 4) || !aligned(grad_weights, 4))
     return misaligned();
   const auto fits = [&](int w) {
     return cols % w == 0 && grad_out_stride % w == 0 && aligned(grad_out, w * es) && aligned(rows, w * es) &&
@@ -1368,8 +1371,8 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   p.rows = static_cast<const char*>(rows);
   p.positions = positions;
   p.weights = weights;
-  p.counts = counts;
   p.offsets = offsets;
+  p.ends = ends;
   p.grad_rows = static_cast<char*>(grad_rows);
   p.grad_weights = grad_weights;
   p.slots = tokens * k;

@@ -789,6 +789,8 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
     return report_error(DGN_ERR_ARG, "dgn_rms_norm: null pointer");
   if (x_stride < cols || (residual && (residual_stride < cols || hidden_stride < cols)))
     return report_error(DGN_ERR_ARG, "a row stride is shorter than the row");
+  if (residual && hidden == residual && hidden_stride != residual_stride)
+    return report_error(DGN_ERR_ARG, "in place, hidden has the residual's stride");
   const int es = (int)dgn_dtype_size(dtype), elems = 16 / es;
   const size_t ws = weight_dtype == DGN_F32 ? 4 : es;
   if (!aligned(x, es) || !aligned(residual, es) || !aligned(hidden, es) || !aligned(out, code ? 1 : es) ||
@@ -863,10 +865,10 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   const size_t ws = weight_dtype == DGN_F32 ? 4 : es;
   if (grad_weight && !aligned(grad_weight, ws))
     return report_error(DGN_ERR_ARG, "a pointer is not aligned to its element size");
-  OnDevice on(device);
-  if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()));
   if (rows == 0) {
     if (!grad_weight) return DGN_OK;
+    OnDevice on(device);
+    if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()));
     cudaError_t e = cudaMemsetAsync(grad_weight, 0, (size_t)cols * ws, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? DGN_OK : report_error(DGN_ERR_CUDA, cudaGetErrorString(e));
   }
@@ -905,6 +907,8 @@ extern "C" int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, 
   p.hidden_stride = hidden_stride;
   p.cols = (int)cols;
   p.weight_f32 = weight_dtype == DGN_F32;
+  OnDevice on(device);
+  if (on.error() != cudaSuccess) return report_error(DGN_ERR_CUDA, cudaGetErrorString(on.error()));
   const bool residual = grad_hidden != nullptr;
   const void* fn = dtype == DGN_F32   ? norm_grad_kernel<float>(s, word, residual)
                    : dtype == DGN_F16 ? norm_grad_kernel<__half>(s, word, residual)

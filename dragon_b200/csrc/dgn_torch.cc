@@ -250,7 +250,7 @@ Tensor route_grad(const Tensor& grad_weights, const Tensor& logits, const Tensor
   return grad;
 }
 
-std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& indices, int64_t experts, int64_t align) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> plan(const Tensor& indices, int64_t experts, int64_t align) {
   if (indices.scalar_type() != ScalarType::Int) unsupported("indices", indices.scalar_type());
   matrix(indices, "indices", true);
   if (!indices.is_contiguous()) value_error("<indices> must be contiguous");
@@ -260,32 +260,31 @@ std::tuple<Tensor, Tensor, Tensor> plan(const Tensor& indices, int64_t experts, 
   if (align < 1 || align > INT32_MAX || slots > INT32_MAX || slots + std::min(experts, slots) * (align - 1) > INT32_MAX)
     value_error("<align> must be positive and the rows fewer than 2^31");
   Tensor counts = empty({experts}, ScalarType::Int, indices), offsets = empty({experts + 1}, ScalarType::Int, indices),
-         positions = empty({tokens, k}, ScalarType::Int, indices), workspace;
+         ends = empty({experts}, ScalarType::Int, indices), positions = empty({tokens, k}, ScalarType::Int, indices), workspace;
   const int64_t bytes = dgn_expert_plan_workspace(slots, (int)experts);
   if (bytes) workspace = empty({bytes}, ScalarType::Byte, indices);
   check(dgn_expert_plan(indices.const_data_ptr<int>(), slots, (int)experts, (int)align, counts.mutable_data_ptr<int>(),
-                        offsets.mutable_data_ptr<int>(), positions.mutable_data_ptr<int>(),
+                        offsets.mutable_data_ptr<int>(), ends.mutable_data_ptr<int>(), positions.mutable_data_ptr<int>(),
                         bytes ? workspace.mutable_data_ptr() : nullptr, bytes, indices.device().index(),
                         stream_of(indices)));
-  return {counts, offsets, positions};
+  return {counts, offsets, ends, positions};
 }
 
 // A plan's tensors, as plan() made them.
 struct Plan {
-  Tensor counts, offsets, positions;
-  int64_t capacity;
+  const Tensor &offsets, &ends, &positions;
   int64_t tokens() const { return positions.size(0); }
   int64_t k() const { return positions.size(1); }
-  int experts() const { return (int)counts.size(0); }
+  int experts() const { return (int)ends.size(0); }
 };
 void check_plan(const Plan& p, const Tensor& like) {
   if (p.positions.device() != like.device())
     value_error("the plan must live on " + like.device().str() + " (got " + p.positions.device().str() + ")");
 }
 
-Tensor dispatch(const Tensor& x, const Tensor& counts, const Tensor& offsets, const Tensor& positions, int64_t capacity,
+Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& ends, const Tensor& positions, int64_t capacity,
                 const MaybeTensor& to) {
-  const Plan p = {counts, offsets, positions, capacity};
+  const Plan p = {offsets, ends, positions};
   const int64_t stride = matrix(x, "x", true), tokens = x.size(0), cols = x.size(1), size = x.element_size();
   check_plan(p, x);
   if (tokens != p.tokens())
@@ -297,7 +296,7 @@ Tensor dispatch(const Tensor& x, const Tensor& counts, const Tensor& offsets, co
   }
   Tensor out = to ? *to : empty({capacity, cols}, x.scalar_type(), x);
   check(dgn_expert_dispatch(x.const_data_ptr(), stride * size, cols * size, positions.const_data_ptr<int>(),
-                            counts.const_data_ptr<int>(), offsets.const_data_ptr<int>(), out.mutable_data_ptr(), tokens,
+                            offsets.const_data_ptr<int>(), ends.const_data_ptr<int>(), out.mutable_data_ptr(), tokens,
                             (int)p.k(), p.experts(), out.size(0), x.device().index(), stream_of(x)));
   return out;
 }
@@ -319,9 +318,9 @@ int64_t of_tokens(const Tensor& t, const Tensor& rows, const Plan& p, const char
   return stride;
 }
 
-Tensor combine(const Tensor& rows, const Tensor& counts, const Tensor& offsets, const Tensor& positions,
+Tensor combine(const Tensor& rows, const Tensor& offsets, const Tensor& ends, const Tensor& positions,
                const MaybeTensor& weights, const MaybeTensor& residual) {
-  const Plan p = {counts, offsets, positions, 0};
+  const Plan p = {offsets, ends, positions};
   const int64_t cols = check_rows(rows, p);
   if (weights) check_exactly(*weights, rows, {p.tokens(), p.k()}, ScalarType::Float, "weights");
   const int64_t residual_stride = residual ? of_tokens(*residual, rows, p, "residual") : 0;
@@ -332,10 +331,10 @@ Tensor combine(const Tensor& rows, const Tensor& counts, const Tensor& offsets, 
   return out;
 }
 
-std::tuple<Tensor, Tensor> combine_grad(const Tensor& grad_output, const Tensor& rows, const Tensor& counts,
-                                        const Tensor& offsets, const Tensor& positions, const Tensor& weights,
+std::tuple<Tensor, Tensor> combine_grad(const Tensor& grad_output, const Tensor& rows, const Tensor& offsets,
+                                        const Tensor& ends, const Tensor& positions, const Tensor& weights,
                                         const MaybeTensor& to) {
-  const Plan p = {counts, offsets, positions, 0};
+  const Plan p = {offsets, ends, positions};
   const int64_t cols = check_rows(rows, p), stride = of_tokens(grad_output, rows, p, "grad_output");
   check_exactly(weights, rows, {p.tokens(), p.k()}, ScalarType::Float, "weights");
   if (to) check_exactly(*to, rows, rows.sizes(), rows.scalar_type(), "out");
@@ -343,7 +342,7 @@ std::tuple<Tensor, Tensor> combine_grad(const Tensor& grad_output, const Tensor&
          grad_weights = empty(weights.sizes(), ScalarType::Float, rows);
   check(dgn_expert_combine_grad(grad_output.const_data_ptr(), stride, rows.const_data_ptr(),
                                 positions.const_data_ptr<int>(), weights.const_data_ptr<float>(),
-                                counts.const_data_ptr<int>(), offsets.const_data_ptr<int>(), out.mutable_data_ptr(),
+                                offsets.const_data_ptr<int>(), ends.const_data_ptr<int>(), out.mutable_data_ptr(),
                                 grad_weights.mutable_data_ptr<float>(), p.tokens(), (int)p.k(), p.experts(), cols,
                                 rows.size(0), dgn_type(rows.scalar_type()), rows.device().index(), stream_of(rows)));
   return {out, grad_weights};

@@ -68,15 +68,16 @@ def route_grad(grad_weights, logits, indices, scores="softmax", renormalize=True
 class ExpertPlan(object):
     """Where the rows of a batch go, all on the device (int32):
 
-    counts [experts], the rows of each expert; offsets [experts + 1], the first
+    counts [experts], the rows of each expert (the caller's to change: an
+    all-reduce may add up the group's in place); offsets [experts + 1], the first
     row of each expert's block, a multiple of `align`, and the end of the last;
-    positions [tokens, k], the row of each choice, -1 for none.  `capacity` is the
+    ends [experts], behind the last row in use of each block; positions [tokens, k], the row of each choice, -1 for none.  `capacity` is the
     number of rows that always suffices."""
 
-    def __init__(self, counts, offsets, positions, align):
-        self.counts, self.offsets, self.positions, self.align = counts, offsets, positions, align
+    def __init__(self, counts, offsets, ends, positions, align):
+        self.counts, self.offsets, self.ends, self.positions, self.align = counts, offsets, ends, positions, align
         self.tokens, self.k = positions.shape
-        self.num_experts = counts.shape[0]
+        self.num_experts = ends.shape[0]
         slots = self.tokens * self.k
         self.capacity = slots + min(self.num_experts, slots) * (align - 1)
 
@@ -102,7 +103,7 @@ def dispatch(x, plan, out=None, stream=None):
     if stream is not None:
         with _enter_stream(stream, x.device):
             return dispatch(x, plan, out)
-    return _C.torch_ops().dispatch(x, plan.counts, plan.offsets, plan.positions, plan.capacity, out)
+    return _C.torch_ops().dispatch(x, plan.offsets, plan.ends, plan.positions, plan.capacity, out)
 
 
 def combine(rows, plan, weights=None, residual=None, stream=None):
@@ -114,7 +115,7 @@ def combine(rows, plan, weights=None, residual=None, stream=None):
     if stream is not None:
         with _enter_stream(stream, rows.device):
             return combine(rows, plan, weights, residual)
-    return _C.torch_ops().combine(rows, plan.counts, plan.offsets, plan.positions, weights, residual)
+    return _C.torch_ops().combine(rows, plan.offsets, plan.ends, plan.positions, weights, residual)
 
 
 def dispatch_grad(grad_rows, plan, stream=None):
@@ -131,7 +132,7 @@ def combine_grad(grad_output, rows, plan, weights, out=None, stream=None):
     if stream is not None:
         with _enter_stream(stream, rows.device):
             return combine_grad(grad_output, rows, plan, weights, out)
-    return _C.torch_ops().combine_grad(grad_output, rows, plan.counts, plan.offsets, plan.positions, weights, out)
+    return _C.torch_ops().combine_grad(grad_output, rows, plan.offsets, plan.ends, plan.positions, weights, out)
 
 
 def update_bias(bias, counts, rate, out=None, stream=None):

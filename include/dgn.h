@@ -368,8 +368,8 @@ int dgn_allreduce_static_status(int clear);
  * hidden is x itself and not written), rstd = 1/sqrt(mean(hidden^2) + eps),
  * out = hidden * rstd * weight.  dtype: DGN_F16, DGN_BF16, DGN_F32; 1..32768
  * columns.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
- * be the residual's own memory with the same stride.  The sum of squares is
- * held in float32.  With a code, out holds 8-bit values instead and scales one
+ * be the residual's own memory, with the same stride.  The sum of squares is
+ * held in float32: a row whose mean square passes 3.4e38 comes out as zeros.  With a code, out holds 8-bit values instead and scales one
  * float32 per row and group of `group` columns (32, 64, 128, or 0: the row):
  * value = code * scale, scale = largest magnitude / largest code (127, 448,
  * 57344), groups below 2^-40 taking that bound's scale; a group with a NaN or an
@@ -420,20 +420,20 @@ int dgn_route_grad(const float* grad_weights, const void* logits, int64_t stride
 /* dgn_expert_plan: where each of the `slots` = tokens * k (token, choice) pairs
  * goes when rows are put in the order of their experts, equal ones in the order
  * of the slots.  Expert e's rows start at offsets[e], a multiple of `align`;
- * counts[e] of them are in use, offsets[e+1] begins the next block and
- * offsets[experts] ends the last.  positions[slot] is -1 for an index outside
+ * counts[e] of them are in use, the last before ends[e] = offsets[e] + counts[e];
+ * offsets[e+1] begins the next block and offsets[experts] ends the last.  positions[slot] is -1 for an index outside
  * 0..experts-1.  slots + min(experts, slots) * (align - 1) rows suffice (below
  * 2^31).  `workspace`: dgn_expert_plan_workspace bytes (may be 0). */
 int64_t dgn_expert_plan_workspace(int64_t slots, int experts);
 int dgn_expert_plan(const int32_t* indices, int64_t slots, int experts, int align, int32_t* counts, int32_t* offsets,
-                    int32_t* positions, void* workspace, int64_t workspace_bytes, int device, void* stream);
+                    int32_t* ends, int32_t* positions, void* workspace, int64_t workspace_bytes, int device, void* stream);
 
 /* out[positions[t*k+j]] = x[t] for rows of row_bytes bytes (any type), x_stride
  * bytes apart in x and contiguous in out, which has `capacity` rows.  The unused
  * rows of each expert's block become zeros, rows behind the last block stay as
  * they are.  A position outside 0..capacity-1 is passed over. */
 int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_bytes, const int32_t* positions,
-                        const int32_t* counts, const int32_t* offsets, void* out, int64_t tokens, int k, int experts,
+                        const int32_t* offsets, const int32_t* ends, void* out, int64_t tokens, int k, int experts,
                         int64_t capacity, int device, void* stream);
 
 /* out[t] = residual[t] + sum over j of weights[t*k+j] * rows[positions[t*k+j]]:
@@ -449,8 +449,8 @@ int dgn_expert_combine(const void* rows, const int32_t* positions, const float* 
  * <grad_out[t], rows[position]>, 0 where there is no position.  A position must
  * stand for one slot only. */
 int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_stride, const void* rows,
-                            const int32_t* positions, const float* weights, const int32_t* counts,
-                            const int32_t* offsets, void* grad_rows, float* grad_weights, int64_t tokens, int k,
+                            const int32_t* positions, const float* weights, const int32_t* offsets,
+                            const int32_t* ends, void* grad_rows, float* grad_weights, int64_t tokens, int k,
                             int experts, int64_t cols, int64_t capacity, int dtype, int device, void* stream);
 
 /* out[e] = bias[e] + rate * sign(mean(counts) - counts[e]): experts that had

@@ -91,7 +91,8 @@ def check_route(logits, k, **kwargs):
 CHOICES = [  # experts, k, groups, keep, best
     (1, 1, 1, 1, 1), (2, 1, 1, 1, 1), (7, 7, 1, 1, 1), (32, 4, 1, 1, 1), (33, 5, 1, 1, 1), (64, 6, 8, 3, 1), (64, 8, 4, 2, 2),
     (96, 32, 1, 1, 1), (128, 8, 1, 1, 1), (160, 6, 32, 9, 2), (256, 8, 8, 4, 2), (257, 9, 1, 1, 1), (384, 8, 2, 1, 2),
-    (512, 10, 4, 3, 1), (600, 3, 3, 2, 2), (1024, 32, 1, 1, 1), (1024, 8, 32, 4, 2)]
+    (512, 10, 4, 3, 1), (600, 3, 3, 2, 2), (1024, 32, 1, 1, 1), (1024, 8, 32, 4, 2), (96, 8, 3, 2, 2), (96, 4, 6, 3, 1),
+    (48, 4, 2, 1, 2), (192, 6, 6, 2, 2), (320, 8, 5, 3, 2), (24, 3, 3, 1, 2)]
 
 
 @pytest.mark.parametrize("num,k,groups,keep,best", CHOICES)
@@ -274,6 +275,7 @@ def test_plan(dgn_lib, tokens, k, num, align):
     counts, offsets, positions = plan_reference(indices, num, align)
     assert p.counts.tolist() == counts
     assert p.offsets.tolist() == offsets
+    assert p.ends.tolist() == [a + n for a, n in zip(offsets, counts)]
     assert p.positions.reshape(-1).tolist() == positions
     assert offsets[-1] <= p.capacity
 
@@ -377,6 +379,18 @@ def test_combine_and_its_gradient(dgn_lib, tokens, k, num, cols, align, dtype):
     assert torch.equal(new_rows[:n], grad_rows[:n]) and torch.equal(new_weights, grad_weights)
 
 
+def test_counts_are_the_callers_to_change(dgn_lib):
+    """The group's counts may be added up in place before the rows move."""
+    p = plan(choices(30, 2, 5, seed=1), 5, 8)
+    n, x, weights = int(p.offsets[-1]), normal(30, 12, seed=2), normal(30, 2, seed=3)
+    want = dispatch(x, p)
+    grads = combine_grad(x, want, p, weights)
+    p.counts.mul_(1000)
+    ones = torch.ones(p.capacity, 12, device=DEV)
+    assert torch.equal(dispatch(x, p, out=ones.clone())[:n], want[:n])
+    assert torch.equal(combine_grad(x, want, p, weights, out=ones)[0][:n], grads[0][:n])
+
+
 def test_combine_of_strided_tensors(dgn_lib):
     p = plan(choices(40, 3, 6, seed=1), 6)
     for dtype in FLOATS:
@@ -463,6 +477,12 @@ def test_refusals_on_the_device(dgn_lib):
         combine(x, p, residual=x.half())
     with pytest.raises(TypeError):
         dispatch(x, p, out=torch.empty(8, 16, device=DEV, dtype=torch.float16))
+
+
+def test_a_stream_of_no_use_is_refused(dgn_lib):
+    x = torch.ones(4, 8)
+    with pytest.raises((ValueError, RuntimeError)):
+        route(x, 2, stream=torch.cuda.Stream())
 
 
 def test_empty_batches(dgn_lib):

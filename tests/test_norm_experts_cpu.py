@@ -49,7 +49,7 @@ def norm_args(**change):
     (dict(weight_dtype=_C.F16), _C.ERR_ARG), (dict(x=None), _C.ERR_ARG), (dict(out=None), _C.ERR_ARG),
     (dict(rstd=None), _C.ERR_ARG), (dict(hidden=None), _C.ERR_ARG), (dict(code=2, scales=None), _C.ERR_ARG),
     (dict(x_stride=63), _C.ERR_ARG), (dict(hidden_stride=63), _C.ERR_ARG), (dict(x=P + 1), _C.ERR_ARG),
-    (dict(weight=P + 2), _C.ERR_ARG), (dict(rstd=P + 2), _C.ERR_ARG)])
+    (dict(weight=P + 2), _C.ERR_ARG), (dict(rstd=P + 2), _C.ERR_ARG), (dict(hidden_stride=72), _C.ERR_ARG)])
 def test_norm_refuses(dgn_lib, change, status):
     assert dgn_lib.dgn_rms_norm(*norm_args(**change)) == status
     assert dgn_lib.dgn_last_error_string()
@@ -69,7 +69,8 @@ def norm_grad_args(**change):
 
 @pytest.mark.parametrize("change,status", [
     (dict(dtype=_C.F64), _C.ERR_UNSUPPORTED), (dict(cols=40000), _C.ERR_ARG), (dict(weight=None), _C.ERR_ARG),
-    (dict(weight_dtype=_C.F16), _C.ERR_ARG), (dict(grad_weight=P + 2), _C.ERR_ARG)])
+    (dict(weight_dtype=_C.F16), _C.ERR_ARG), (dict(grad_weight=P + 2), _C.ERR_ARG),
+    (dict(workspace_bytes=4), _C.ERR_ARG), (dict(rstd=None), _C.ERR_ARG), (dict(grad_hidden_stride=63), _C.ERR_ARG)])
 def test_norm_grad_refuses(dgn_lib, change, status):
     assert dgn_lib.dgn_rms_norm_grad(*norm_grad_args(**change)) == status
 
@@ -112,7 +113,7 @@ def test_calls_without_tokens_do_nothing(dgn_lib):
     (-1, 8, 1, 0, _C.ERR_ARG), (1 << 31, 8, 1, 0, _C.ERR_ARG), (8, 0, 1, 0, _C.ERR_ARG), (8, 1025, 1, 0, _C.ERR_ARG),
     (8, 8, 0, 0, _C.ERR_ARG), (1 << 20, 8, 1 << 30, 0, _C.ERR_ARG), (1 << 20, 8, 1, 0, _C.ERR_ARG)])
 def test_plan_refuses(dgn_lib, slots, num, align, ws, status):
-    assert dgn_lib.dgn_expert_plan(P, slots, num, align, P, P, P, None, ws, 0, None) == status
+    assert dgn_lib.dgn_expert_plan(P, slots, num, align, P, P, P, P, None, ws, 0, None) == status
 
 
 def test_moves_refuse(dgn_lib):
