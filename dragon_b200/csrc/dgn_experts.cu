@@ -693,7 +693,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanBlocks = 148;
+constexpr int kSMs = 148;
+constexpr int kPlanBlocks = kSMs;
 // Slots that one block counts before another joins: 65536 slots of 64 experts take 8.5 us with 2048, 9.4 with 1024, 9.8 with 4096.
 constexpr int kSlotsOfBlock = 2048;
 
@@ -850,7 +851,8 @@ __global__ void __launch_bounds__(kMoveThreads) dispatch_kernel(const __grid_con
   __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
   const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
   const long long t = (long long)(blockIdx.x - p.experts) * (kMoveThreads / TEAM) + team;
-  if (t < p.tokens && me < p.k) place[team][me] = p.positions[t * p.k + me];
+  if (t < p.tokens)
+    for (int j = me; j < p.k; j += TEAM) place[team][j] = p.positions[t * p.k + j];
   if (TEAM > 32) __syncthreads();
   else __syncwarp();
   if (t >= p.tokens) return;
@@ -1073,8 +1075,14 @@ const void* route_grad_fn(int experts) {
   if (experts <= 512) return (const void*)route_grad_kernel<T, 32, 16, VEC>;
   return (const void*)route_grad_kernel<T, 32, 32, VEC>;
 }
-// Threads for a token's row of `words` words, of which each thread takes about four.
-int move_team(int64_t words) { return words <= 128 ? 32 : words <= 512 ? 128 : 256; }
+// Threads for a token's row of `words` words, of which each thread takes about four (one where rows are narrow); more
+// threads while the tokens do not fill two blocks on each SM.
+int move_team(int64_t words, int64_t tokens) {
+  const int sizes[] = {8, 32, 128, 256};
+  int i = words <= 16 ? 0 : words <= 128 ? 1 : words <= 512 ? 2 : 3;
+  while (i < 3 && words > sizes[i] && tokens * sizes[i] < 2 * kMoveThreads * kSMs) ++i;
+  return sizes[i];
+}
 
 // The same for a sum of rows, of which each thread takes two parts (one where a warp would be half idle).
 struct CombineTeam {
@@ -1086,7 +1094,8 @@ CombineTeam combine_team(int64_t parts) {
 
 template <typename U>
 const void* dispatch_fn(int team) {
-  return team == 32    ? (const void*)dispatch_kernel<U, 32>
+  return team == 8     ? (const void*)dispatch_kernel<U, 8>
+         : team == 32  ? (const void*)dispatch_kernel<U, 32>
          : team == 128 ? (const void*)dispatch_kernel<U, 128>
                        : (const void*)dispatch_kernel<U, 256>;
 }
@@ -1295,7 +1304,7 @@ extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_
   p.experts = experts;
   // The widest word that divides the addresses, the strides and the row.
   const auto fits = [&](int w) { return aligned(x, w) && aligned(out, w) && x_stride % w == 0 && row_bytes % w == 0; };
-  const int word = fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1, team = move_team(row_bytes / word);
+  const int word = fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1, team = move_team(row_bytes / word, tokens);
   const void* fn = word == 16  ? dispatch_fn<uint4>(team)
                    : word == 8 ? dispatch_fn<uint2>(team)
                    : word == 4 ? dispatch_fn<unsigned>(team)
