@@ -250,6 +250,11 @@ __device__ __forceinline__ float quick_exp(float x) {
   return r;
 }
 
+__device__ __forceinline__ float larger(float a, float b) {  // a NaN stays one
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 __device__ __forceinline__ float quick_reciprocal(float x) {  // to one step
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -350,17 +355,15 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
 
   float x[N];
   load_logits<T, L, N, VEC>(row, live, experts, lane, x);
-  bool odd = false;  // what float32 does not decide
+  float peak = x[0];  // a NaN stays one
 #pragma unroll
-  for (int i = 0; i < N; ++i) odd |= !(x[i] < INFINITY);
+  for (int i = 1; i < N; ++i) peak = larger(peak, x[i]);
+  bool odd = !(peak < INFINITY);  // what float32 does not decide
   // Scores of all experts are needed with a bias, and their sum unless it cancels in the weights.
   const bool plain = !p.bias && p.groups == 1;
   float top = 0.f, inv = 1.f, largest_score = 1.f;
   if (!p.sigmoid && !(plain && p.renormalize)) {
-    top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
-    top = team_max<L>(top);
+    top = team_max<L>(peak);
     if (top == -INFINITY) top = 0.f;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -375,11 +378,13 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
   if (p.bias) {  // from here on x is the key
     float b[N];
     load_logits<float, L, N, VEC, 16 / (int)sizeof(T)>(p.bias, live, experts, lane, b);
+    peak = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (x[i] > -INFINITY) x[i] = score_of(x[i]) + b[i];
-      odd |= !(x[i] < INFINITY);
+      peak = larger(peak, x[i]);
     }
+    odd |= !(peak < INFINITY);
   }
 
   if (p.groups > 1) {
@@ -474,14 +479,14 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
   }
 
   // Words: the upper bits of the key's order, or of its place between the largest and the smallest key.
-  unsigned word[N], need = 1;  // need: how many steps apart two words have to be
+  // need: how many steps apart two words have to be; least_word: words below it stand for -inf, which comes before the
+  // order of the lowest number.
+  unsigned word[N], need = 1, least_word = 1u << 22;
   if (!p.bias) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = expert_of<T, L, VEC>(i, lane);
-      word[i] = x[i] > -INFINITY ? (order_of(x[i]) >> 1 & ~low) | (low - e) : 0;
-    }
+    for (int i = 0; i < N; ++i) word[i] = (order_of(x[i]) >> 1 & ~low) + (low - expert_of<T, L, VEC>(i, lane));
   } else {
+    least_word = 1;
     float most = -INFINITY, least = INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
     for (int i = 0; i < N; ++i) best = __viaddmax_u32(word[i], -last, best);
     best = best >= kWrap ? best + last : 0;
     last = team_max<L>(best);
-    if (lane == j % L) win[j] = last;
+    if (lane == j % L) win[j] = last < least_word ? 0 : last;
     if (last == 0) last = 1;  // nothing is left: only zeros stay below
   };
   const bool certain = sizeof(T) == 2 && !p.bias;
