@@ -829,38 +829,76 @@ struct MoveParams {
   const int* ends;
   char* out;
   long long tokens, x_stride, row_bytes, capacity;  // bytes
-  int k, experts;
+  int k, experts, share;  // share: blocks for the unused rows of an expert
 };
 
-// Zeros in the rows of an expert's block that no slot uses, by a whole block of threads.
-// Such blocks come first in the grid: behind the others they would be its tail.
-template <typename U>
-__device__ void clear_rows(char* out, const int* offsets, const int* ends, int e, long long row_bytes,
+// Zeros in the rows of an expert's block that no slot uses, by `share` blocks of threads.
+// They lie in one piece, so they are written by 16 bytes whatever the row.  Such blocks come first in
+// the grid: behind the others they would be its tail.
+__device__ void clear_rows(char* out, const int* offsets, const int* ends, int block, int share, long long row_bytes,
                            long long capacity) {
+  const int e = block / share;
   const long long first = max(0, ends[e]), last = min((long long)offsets[e + 1], capacity);
   if (first >= last) return;
-  U* to = reinterpret_cast<U*>(out + first * row_bytes);
-  const long long n = (last - first) * row_bytes / (long long)sizeof(U);
+  char* begin = out + first * row_bytes;
+  const long long bytes = (last - first) * row_bytes;
+  const long long head = min((long long)(-reinterpret_cast<uintptr_t>(begin) & 15), bytes), n = (bytes - head) / 16;
+  uint4* body = reinterpret_cast<uint4*>(begin + head);
 #pragma unroll 4
-  for (long long i = threadIdx.x; i < n; i += kMoveThreads) to[i] = U{};
+  for (long long i = (long long)(block % share) * kMoveThreads + threadIdx.x; i < n; i += (long long)share * kMoveThreads)
+    body[i] = make_uint4(0, 0, 0, 0);
+  if (block % share) return;
+  if (threadIdx.x < head) begin[threadIdx.x] = 0;
+  if (threadIdx.x < bytes - head - n * 16) begin[head + n * 16 + threadIdx.x] = 0;
+}
+
+// Bytes q .. q + 15 of the 32 bytes {lo, hi}; 0 < q < 16.
+__device__ __forceinline__ uint4 shift16(uint4 lo, uint4 hi, unsigned q) {
+  unsigned w0 = lo.x, w1 = lo.y, w2 = lo.z, w3 = lo.w, w4 = hi.x, w5 = hi.y, w6 = hi.z;
+  if (q & 8) { w0 = w2; w1 = w3; w2 = w4; w3 = w5; w4 = w6; w5 = hi.w; }
+  if (q & 4) { w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5; }
+  const unsigned bits = (q & 3) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
+}
+
+// Copies a row between any two addresses by TEAM threads: the aligned vectors of the target are made of the two aligned
+// vectors of the source around them (each holds a byte of the row: nothing else is mapped in), its ends byte by byte.
+template <int TEAM>
+__device__ __forceinline__ void copy_row(char* to, const char* from, int bytes, int me) {
+  const int head = min((int)(-reinterpret_cast<uintptr_t>(to) & 15), bytes), n = (bytes - head) / 16;
+  for (int i = me; i < head; i += TEAM) to[i] = from[i];
+  for (int i = head + n * 16 + me; i < bytes; i += TEAM) to[i] = from[i];
+  const unsigned q = (unsigned)(reinterpret_cast<uintptr_t>(from + head) & 15);
+  const uint4* source = reinterpret_cast<const uint4*>(from + head - q);
+  uint4* target = reinterpret_cast<uint4*>(to + head);
+#pragma unroll 2
+  for (int i = me; i < n; i += TEAM) target[i] = q ? shift16(source[i], source[i + 1], q) : source[i];
 }
 
 // TEAM threads for a token: four words of its row at a time are read once and written to
-// each of its k places.
+// each of its k places.  Rows that no word of 4 bytes divides (U a byte) are copied to each place by themselves.
 template <typename U, int TEAM>
 __global__ void __launch_bounds__(kMoveThreads) dispatch_kernel(const __grid_constant__ MoveParams p) {
-  if (blockIdx.x < p.experts) {
-    clear_rows<U>(p.out, p.offsets, p.ends, blockIdx.x, p.row_bytes, p.capacity);
+  if (blockIdx.x < p.experts * p.share) {
+    clear_rows(p.out, p.offsets, p.ends, blockIdx.x, p.share, p.row_bytes, p.capacity);
     return;
   }
   __shared__ int place[kMoveThreads / TEAM][kMaxChoices];
   const int team = threadIdx.x / TEAM, me = threadIdx.x % TEAM;
-  const long long t = (long long)(blockIdx.x - p.experts) * (kMoveThreads / TEAM) + team;
+  const long long t = (long long)(blockIdx.x - p.experts * p.share) * (kMoveThreads / TEAM) + team;
   if (t < p.tokens)
     for (int j = me; j < p.k; j += TEAM) place[team][j] = p.positions[t * p.k + j];
   if (TEAM > 32) __syncthreads();
   else __syncwarp();
   if (t >= p.tokens) return;
+  if constexpr (sizeof(U) == 1) {
+    for (int j = 0; j < p.k; ++j) {
+      const int at = place[team][j];
+      if (at >= 0 && at < p.capacity) copy_row<TEAM>(p.out + at * p.row_bytes, p.x + t * p.x_stride, (int)p.row_bytes, me);
+    }
+    return;
+  }
   const U* from = reinterpret_cast<const U*>(p.x + t * p.x_stride);
   const long long n = p.row_bytes / (long long)sizeof(U);
   for (long long base = me; base < n; base += 4 * TEAM) {
@@ -990,7 +1028,7 @@ struct CombineGradParams {
   char* grad_rows;
   float* grad_weights;
   long long slots, capacity, grad_out_stride;
-  int cols, k, experts;
+  int cols, k, experts, share;
 };
 
 // A warp for a slot: no warp waits for another.  The slots of a token are neighbours, so its
@@ -999,11 +1037,11 @@ template <typename T, int W>
 __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid_constant__ CombineGradParams p) {
   constexpr int E = Elem<T>::E, AHEAD = 4;
   const long long row_bytes = p.cols * (long long)sizeof(T);
-  if (blockIdx.x < p.experts) {
-    clear_rows<typename Word<W * sizeof(T)>::type>(p.grad_rows, p.offsets, p.ends, blockIdx.x, row_bytes, p.capacity);
+  if (blockIdx.x < p.experts * p.share) {
+    clear_rows(p.grad_rows, p.offsets, p.ends, blockIdx.x, p.share, row_bytes, p.capacity);
     return;
   }
-  const long long slot = (long long)(blockIdx.x - p.experts) * (kMoveThreads / 32) + (threadIdx.x >> 5);
+  const long long slot = (long long)(blockIdx.x - p.experts * p.share) * (kMoveThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (slot >= p.slots) return;
   const long long at = p.positions[slot];
@@ -1080,6 +1118,13 @@ const void* route_grad_fn(int experts) {
   if (experts <= 512) return (const void*)route_grad_kernel<T, 32, 16, VEC>;
   return (const void*)route_grad_kernel<T, 32, 32, VEC>;
 }
+// Blocks that clear the unused rows of one expert: one for each 128 KB that the rows beyond the slots may take for it.
+int clear_share(int64_t slots, int experts, int64_t capacity, int64_t row_bytes) {
+  const int64_t spare = capacity > slots ? (capacity - slots) * row_bytes : 0, each = slots < experts ? slots : experts;
+  const int64_t share = ceil_div(spare, each * (128 << 10));
+  return (int)(share < 1 ? 1 : share > 16 ? 16 : share);
+}
+
 // Threads for a token's row of `words` words, of which each thread takes about four (one where rows are narrow); more
 // threads while the tokens do not fill two blocks on each SM.
 int move_team(int64_t words, int64_t tokens) {
@@ -1309,15 +1354,16 @@ extern "C" int dgn_expert_dispatch(const void* x, int64_t x_stride, int64_t row_
   p.experts = experts;
   // The widest word that divides the addresses, the strides and the row.
   const auto fits = [&](int w) { return aligned(x, w) && aligned(out, w) && x_stride % w == 0 && row_bytes % w == 0; };
-  const int word = fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1, team = move_team(row_bytes / word, tokens);
+  const int word = fits(16) ? 16 : fits(8) ? 8 : fits(4) ? 4 : 1;
+  const int team = move_team(word == 1 ? ceil_div(row_bytes, 16) : row_bytes / word, tokens);
+  p.share = clear_share(tokens * k, experts, capacity, row_bytes);
   const void* fn = word == 16  ? dispatch_fn<uint4>(team)
                    : word == 8 ? dispatch_fn<uint2>(team)
                    : word == 4 ? dispatch_fn<unsigned>(team)
-                   : word == 2 ? dispatch_fn<unsigned short>(team)
                                : dispatch_fn<unsigned char>(team);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)(ceil_div(tokens, kMoveThreads / team) + experts)), dim3(kMoveThreads), 0, stream, args);
+  return launch(fn, dim3((unsigned)(ceil_div(tokens, kMoveThreads / team) + (int64_t)experts * p.share)), dim3(kMoveThreads), 0, stream, args);
 }
 
 extern "C" int dgn_expert_combine(const void* rows, const int32_t* positions, const float* weights,
@@ -1395,12 +1441,13 @@ extern "C" int dgn_expert_combine_grad(const void* grad_out, int64_t grad_out_st
   p.grad_out_stride = grad_out_stride;
   p.k = k;
   p.experts = experts;
+  p.share = clear_share(tokens * k, experts, capacity, cols * es);
   const void* fn = dtype == DGN_F32   ? combine_grad_fn<float>(word)
                    : dtype == DGN_F16 ? combine_grad_fn<__half>(word)
                                       : combine_grad_fn<__nv_bfloat16>(word);
   DGN_ON(device);
   void* args[] = {&p};
-  return launch(fn, dim3((unsigned)(ceil_div(tokens * k, kMoveThreads / 32) + experts)), dim3(kMoveThreads), 0, stream, args);
+  return launch(fn, dim3((unsigned)(ceil_div(tokens * k, kMoveThreads / 32) + (int64_t)experts * p.share)), dim3(kMoveThreads), 0, stream, args);
 }
 
 extern "C" int dgn_expert_update_bias(const float* bias, const int32_t* counts, float* out, int experts, float rate,

@@ -238,7 +238,9 @@ __device__ __forceinline__ float inverse_root(float v) {
 __device__ __forceinline__ float code_factor(float m, float rstd, float largest) {
   const float top = m * rstd;
   if (!(top < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);  // a NaN or an infinity: reads as NaN
-  return top >= kSmallestAmax ? largest * reciprocal(m) : largest * rstd * (1.f / kSmallestAmax);
+  if (top < kSmallestAmax) return largest * rstd * (1.f / kSmallestAmax);
+  const float r = reciprocal(m), f = largest * r;
+  return fmaf(fmaf(-f, m, largest), r, f);  // the quotient, corrected by its remainder
 }
 __device__ __forceinline__ float code_scale(float m, float rstd, float inv_largest) {
   const float top = m * rstd;
