@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
   constexpr int RU = !TEAM || !VEC ? 1 : NV == 1 ? 4 : NV == 2 ? 2 : 1;
   constexpr long long S = sizeof(T);
   __shared__ __align__(16) float slot[2][32];
-  __shared__ float chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
+  __shared__ float chunk[VEC || !CODES ? 1 : 1024], factor[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const long long first = (long long)blockIdx.x * blockDim.y * RU + threadIdx.y;
   uint4 h[RU][NV], r[RU][NV];
@@ -345,18 +345,33 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
 #pragma unroll
           for (int e = 0; e < E; e += W) {  // 32 / W lanes hold a chunk's words
             float m = fabsf(a[e] * w[e]);
-            if (W == 2) m = Largest::of(m, a[e + 1] * w[e + 1]);
+            if (W == 1) {
+              m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // by its bits a NaN is largest
+            } else {
+              m = Largest::of(m, a[e + 1] * w[e + 1]);
 #pragma unroll
-            for (int d = 16 / W; d; d >>= 1) m = Largest::of(m, __shfl_xor_sync(0xffffffffu, m, d));
+              for (int d = 8; d; d >>= 1) m = Largest::of(m, __shfl_xor_sync(0xffffffffu, m, d));
+            }
             const int c = column<T, W>(i, e, me, team);
             if ((c & 31) == 0 && c < cols) chunk[threadIdx.y * 32 + (c >> 5)] = m;
           }
         }
       }
     }
-    if (whole) team_reduce<Largest, TEAM>(top, slot[1]);
-    else if (TEAM) __syncwarp();
-    else __syncthreads();
+    const auto meet = [] { TEAM ? __syncwarp() : __syncthreads(); };
+    if (whole) {
+      team_reduce<Largest, TEAM>(top, slot[1]);
+    } else {
+      meet();
+      const int chunks = (cols + 31) >> 5, of_group = 1 << (p.group_shift - 5);
+      for (int g = me; g < p.groups; g += team) {
+        float m = 0.f;
+        for (int k = g * of_group; k < min((g + 1) * of_group, chunks); ++k) m = Largest::of(m, chunk[threadIdx.y * 32 + k]);
+        factor[threadIdx.y * 32 + g] = code_factor(m, rstd[0], largest);
+        if (first < p.rows) p.scales[first * p.groups + g] = code_scale(m, rstd[0], p.inv_largest);
+      }
+      meet();
+    }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -391,20 +406,12 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
         else *reinterpret_cast<unsigned*>(out + c) = codes.x;
       } else {
         const float all = code_factor(top[u], rstd[u], largest);
+        if (whole && me == 0 && i == 0 && row < p.rows) p.scales[row] = code_scale(top[u], rstd[u], p.inv_largest);
 #pragma unroll
         for (int e = 0; e < E; e += W) {
           const int c = column<T, W>(i, e, me, team);
           if (c >= cols || row >= p.rows) continue;
-          float m = top[u], f = all;
-          int group = 0;
-          if (!whole) {
-            group = c >> p.group_shift;
-            const int begin = group << (p.group_shift - 5), end = min(begin + (1 << (p.group_shift - 5)), (cols + 31) >> 5);
-            m = 0.f;
-            for (int k = begin; k < end; ++k) m = Largest::of(m, chunk[threadIdx.y * 32 + k]);
-            f = code_factor(m, rstd[u], largest);
-          }
-          if (c == (whole ? 0 : group << p.group_shift)) p.scales[row * p.groups + group] = code_scale(m, rstd[u], p.inv_largest);
+          const float f = whole ? all : factor[threadIdx.y * 32 + (c >> p.group_shift)];
           const float2 v = a[e / 2].get();
           if (W == 2)
             *reinterpret_cast<unsigned short*>(out + c) =
