@@ -3,7 +3,11 @@
 // of their experts, the copy of the rows into that order, the weighted sum back
 // with its backward pass, and the update of the balance bias.
 //
-// All are bound by the bytes they move; no matrix product is involved.
+// No matrix product is involved.  The moves are bound by memory: 65536 slots of 2048
+// bfloat16 columns take 50 us to dispatch (93 % of the measured copy rate), 55 to combine with a
+// residual (94 %), 98 for the backward pass (90 %), 48 without weights (98 %).  The choice is
+// bound by its instructions: 65536 tokens of 128 float32 logits take 22 us, the bytes 5.8; its
+// gradient 15.7 of 11.0.
 #include <math.h>
 
 #include "dgn_kernels.cuh"
@@ -700,7 +704,8 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kSMs = 148;
 constexpr int kPlanBlocks = kSMs;
-// Slots that one block counts before another joins: 65536 slots of 64 experts take 8.5 us with 2048, 9.4 with 1024, 9.8 with 4096.
+// Slots that one block counts before another joins.  65536 slots of 64 experts took 8.5 us with 2048, 9.4 with 1024 and 9.8
+// with 4096; 7.1 since the two kernels overlap.
 constexpr int kSlotsOfBlock = 2048;
 
 int plan_blocks(int64_t slots) {

@@ -12,6 +12,13 @@
 //
 // Sums are held in 32 bits.  A row is read once: it stays in registers, packed in
 // its storage type, between the sum of squares and the output.
+//
+// Bound by memory: 8192 rows of 4096 bfloat16 columns with a residual take 42.8 us forward
+// (6.3 TB/s, 97 % of the measured copy rate) and 44.8 us backward (93 %: 41 without the
+// weight gradient, whose partial sums go through the second cache and a second kernel).  With 8-bit output it
+// is the instructions, 42.7 us for bytes of 36.3: each value is rounded, multiplied, compared and
+// converted.  Rows that are not aligned move by single or paired elements and
+// are bound by their number: 4097 columns take 95 us forward, 278 backward.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -552,7 +559,8 @@ __device__ __forceinline__ void copy_async(uint4* to, const char* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
-// Aligned rows.  Each thread copies its own vectors of the rows to come into its own places of a ring in shared memory
+// Aligned rows (8192 x 4096 bfloat16: 41 us of 41.5 at the copy rate, 62 for the plain form with as
+// many blocks).  Each thread copies its own vectors of the rows to come into its own places of a ring in shared memory
 // (cp.async), so the loads of STAGES - 1 rows are in flight while one is worked on and nobody waits for another
 // thread's copy; the sums of the weight gradient (and up to 16 weights a thread) stay in
 // registers for all of the block's rows.
@@ -668,6 +676,7 @@ struct RowShape {
   int lanes() const { return teams > 1 ? team : 0; }  // the kernels' TEAM
 };
 
+// Two parts a thread up to 512: with four, 4096 columns of bfloat16 in 8 bits took 45.0 us instead of 42.6.
 // Rows of up to 128 parts go to a warp or a half or quarter of one and need no barrier; longer ones to a block, with
 // more parts for a thread where the threads would pass 512.
 RowShape row_shape(int cols, int elems, bool vec) {
@@ -681,7 +690,7 @@ RowShape row_shape(int cols, int elems, bool vec) {
 }
 
 // The backward pass keeps the weights and their gradient in registers: two parts a thread wherever 512 threads will do.
-// With four, whose weights are read again for each row, 32768 rows of 1024 bfloat16 columns took 55.7 us instead of 47.9;
+// With four, whose weights are read again for each row, 32768 rows of 1024 bfloat16 columns took 55.7 us instead of 46.7;
 // two for each of 1024 threads spill (2048 rows of 16384 columns: 85 us, 78 with four for 512).
 RowShape grad_shape(int cols, int elems, bool vec) {
   const int parts = (int)ceil_div(cols, elems);
