@@ -21,6 +21,7 @@ class OnDevice {
       err_ = cudaSetDevice(device);
       switched_ = err_ == cudaSuccess;
     }
+    if (err_ != cudaSuccess) cudaGetLastError();
   }
   ~OnDevice() {
     if (switched_) cudaSetDevice(prev_);

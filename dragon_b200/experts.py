@@ -11,8 +11,7 @@ dgn_expert_* of include/dgn.h).
     grad_x = dispatch_grad(grad_rows, p)
     grad_logits = route_grad(grad_weights, logits, indices)
 
-    comm.all_reduce([p.counts])                           # the group's token counts
-    update_bias(bias, p.counts, rate)                     # the same new bias on every rank
+    gradient_sync.sync_expert_bias(bias, p.counts, rate)  # the group's counts, the same new bias on every rank
 
 Like the collectives these calls enqueue work on a stream and return: nothing
 is synchronised, so the number of rows of each expert stays on the device, and

@@ -1,5 +1,6 @@
-"""The two data-parallel gradient-sync call sites of the reference, as
-functions over torch CUDA tensors.
+"""What a data-parallel training step synchronises, as functions over torch CUDA
+tensors: the two gradient-sync call sites of the reference, and the balance
+bias of a layer of experts.
 
 * torch frontend, ``Optimizer.step`` (torch/core/optim/optimizer.py:134-164,
   261-262): gradients are grouped by dtype, each group is all-reduced in place
@@ -10,11 +11,12 @@ functions over torch CUDA tensors.
   one ``Collective`` with ``reduction="MEAN"`` and no bucketing (one collective
   per tensor in the reference; still one operator run here).
 
-Both return without synchronising; the gradients are reduced in place.
+They return without synchronising; the gradients are reduced in place.
 """
 
 import collections
 
+from dragon_b200 import experts
 from dragon_b200.distributed import backend as dist_backend
 from dragon_b200.distributed.ops import _execute
 
@@ -42,3 +44,22 @@ def sync_gradients_native_style(grads, group=None):
     grads = [g for g in grads if g is not None]
     if grads:
         _execute(group, grads, outputs=grads, operation="ALLREDUCE", reduction="MEAN")
+
+
+def sync_expert_bias(bias, counts, rate, group=None):
+    """One step of the balance bias of experts.route(): the ranks' token counts
+    (experts.plan().counts, int32) are summed in place by an all-reduce, and
+    ``bias`` moves by ``rate`` towards the experts that had fewer than the mean, in
+    place and to the same bits on every rank.  Without a group the counts are this
+    process's own; a rank outside of the group leaves both alone.
+
+    Virtual ranks of an emulated world (a collective runs when the last of them
+    issues it) all-reduce first, each of them, and then call experts.update_bias."""
+    group = group or dist_backend.get_group()
+    if group is not None:
+        if dist_backend.communicator(group) is None:
+            return bias
+        if group.size > 1 and isinstance(dist_backend._world(), dist_backend._EmulatedWorld):
+            raise RuntimeError("virtual ranks all-reduce their counts before any of them updates its bias")
+        _execute(group, [counts], outputs=[counts], operation="ALLREDUCE", reduction="SUM")
+    return experts.update_bias(bias, counts, rate)

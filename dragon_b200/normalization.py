@@ -45,7 +45,8 @@ def rms_norm_grad(grad_output, hidden, rstd, weight=None, grad_hidden=None, stre
     8-bit output passes its gradient straight through).  grad_hidden: the
     gradient that reaches `hidden` along the residual, or None.  grad_x is the
     gradient of x and of the residual alike; grad_weight has the weight's type
-    and is None without a weight.  The same inputs give the same bits."""
+    and is None without a weight.  The same inputs in the same layout give
+    the same bits."""
     if stream is not None:
         with _enter_stream(stream, hidden.device):
             return rms_norm_grad(grad_output, hidden, rstd, weight, grad_hidden)

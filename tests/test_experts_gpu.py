@@ -630,6 +630,38 @@ def test_a_layer_of_experts_trains_across_ranks(dgn_lib):
             c.destroy()
 
 
+def test_sync_expert_bias(dgn_lib):
+    """With a group of one, without a group, outside of one, and where virtual ranks would read too early."""
+    from dragon_b200 import distributed
+    from dragon_b200.gradient_sync import sync_expert_bias
+    distributed.finalize()
+    try:
+        for group in (distributed.new_group([0]), None):
+            p = plan(choices(50, 2, 6, seed=3), 6)
+            bias, counts = normal(6, seed=1), p.counts.clone()
+            want = update_bias(bias.clone(), counts, 1e-2)
+            assert sync_expert_bias(bias, p.counts, 1e-2, group) is bias
+            assert torch.equal(bias, want) and torch.equal(p.counts, counts)
+        distributed.init_emulated_world(2, 0)
+        both, other = distributed.new_group([0, 1]), distributed.new_group([1])
+        with distributed.as_rank(0):
+            with pytest.raises(RuntimeError, match="virtual ranks"):
+                sync_expert_bias(bias, p.counts, 1e-2, both)
+            assert torch.equal(sync_expert_bias(bias, p.counts, 1e-2, other), want)  # not a member
+    finally:
+        torch.cuda.synchronize()
+        distributed.finalize()
+
+
+def test_a_device_that_does_not_exist_is_an_error(dgn_lib):
+    from dragon_b200 import _C
+    bias, counts = torch.zeros(4, device=DEV), torch.ones(4, dtype=torch.int32, device=DEV)
+    args = (bias.data_ptr(), counts.data_ptr(), bias.data_ptr(), 4, 0.5)
+    assert dgn_lib.dgn_expert_update_bias(*args, 4096, None) == _C.ERR_CUDA
+    assert dgn_lib.dgn_last_error_string()
+    assert torch.equal(update_bias(bias, counts, 0.5), torch.zeros(4, device=DEV))  # and nothing of it stays behind
+
+
 def test_eight_bit_rows_travel(dgn_lib):
     """The norm's 8-bit rows and scales through all-gather and dispatch stand for the same values."""
     from dragon_b200.comm import Communicator

@@ -154,6 +154,21 @@ def test_strided_rows_and_unaligned_starts(dgn_lib, dtype, cols, offset):
     assert torch.equal(rms_norm(x3).output, rms_norm(x3.view(12, cols)).output.view(3, 4, cols))
 
 
+def test_rows_of_more_dimensions(dgn_lib):
+    """Dimensions that fold into rows at one distance are taken, others refused."""
+    wide = make(12, 100, torch.float32, 7).view(3, 4, 100)
+    cut = wide[:, :, 8:72]
+    r, flat = rms_norm(cut, residual=wide[:, :, 20:84]), rms_norm(cut.reshape(12, 64), residual=wide[:, :, 20:84].reshape(12, 64))
+    assert r.output.shape == (3, 4, 64) and r.rstd.shape == (3, 4)
+    assert torch.equal(r.output.view(12, 64), flat.output) and torch.equal(r.hidden.view(12, 64), flat.hidden)
+    grad, _ = rms_norm_grad(cut, r.hidden, r.rstd)
+    assert torch.equal(grad.view(12, 64), rms_norm_grad(cut.reshape(12, 64), flat.hidden, flat.rstd)[0])
+    for bad in (wide.transpose(0, 1), wide[:, ::3], wide[..., ::2]):
+        with pytest.raises(ValueError):
+            rms_norm(bad)
+    assert rms_norm(make(1, 64, torch.float32, 8)[0]).output.shape == (64,)
+
+
 def grad_reference(dy, hidden, rstd, weight, grad_hidden):
     dy, h, r = dy.double(), hidden.double(), rstd.double()[:, None]
     g = dy if weight is None else dy * weight.double()
