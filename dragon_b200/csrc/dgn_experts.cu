@@ -953,6 +953,29 @@ __device__ __forceinline__ void put(char* row, int i, int me, int cols, uint4 v)
   }
 }
 
+// The same for 16-bit rows that words of two do not divide, whose threads still take E neighbouring elements: the two
+// aligned vectors around them, shifted together (each holds an element of the row).
+template <typename T, int TEAM>
+__device__ __forceinline__ uint4 part_between(const char* row, int i, int me, int cols) {
+  constexpr int E = Elem<T>::E;
+  const int c = (i * TEAM + me) * E, left = cols - c;
+  if (left <= 0) return make_uint4(0, 0, 0, 0);
+  const char* p = row + (size_t)c * sizeof(T);
+  const unsigned q = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4* from = reinterpret_cast<const uint4*>(p - q);
+  uint4 v = from[0];
+  if (q) v = shift16(v, (int)q + left * (int)sizeof(T) > 16 ? from[1] : make_uint4(0, 0, 0, 0), q);
+  return v;  // elements behind the last are the caller's to leave out
+}
+template <typename T, int TEAM>
+__device__ __forceinline__ void put_between(char* row, int i, int me, int cols, uint4 v) {
+  constexpr int E = Elem<T>::E;
+  const int c = (i * TEAM + me) * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (c + e < cols) reinterpret_cast<unsigned short*>(row)[c + e] = reinterpret_cast<const unsigned short*>(&v)[e];
+}
+
 struct CombineParams {
   const char* rows;
   const int* positions;
@@ -980,6 +1003,14 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
   if (TEAM > 32) __syncthreads();
   else __syncwarp();
   if (t >= p.tokens) return;
+  const auto take = [&](const char* row, int i, int thread, int cols) {
+    if constexpr (W == 1 && sizeof(T) == 2) return part_between<T, TEAM>(row, i, thread, cols);
+    else return part<T, W, TEAM>(row, i, thread, cols);
+  };
+  const auto give = [&](char* row, int i, int thread, int cols, uint4 v) {
+    if constexpr (W == 1 && sizeof(T) == 2) put_between<T, TEAM>(row, i, thread, cols, v);
+    else put<T, W, TEAM>(row, i, thread, cols, v);
+  };
   const int parts = (p.cols + TEAM * E - 1) / (TEAM * E);
   for (int i = 0; i < parts; i += TWO) {
     float sum[TWO][E], a[E];
@@ -988,7 +1019,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
     for (int u = 0; u < TWO; ++u) {
 #pragma unroll
       for (int e = 0; e < E; ++e) sum[u][e] = 0.f;
-      if (p.residual) r[u] = part<T, W, TEAM>(p.residual + t * p.residual_stride * (long long)sizeof(T), i + u, me, p.cols);
+      if (p.residual) r[u] = take(p.residual + t * p.residual_stride * (long long)sizeof(T), i + u, me, p.cols);
     }
     for (int j = 0; j < p.k; j += AHEAD) {
       uint4 v[AHEAD][TWO];
@@ -997,7 +1028,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
         if (j + n < p.k && place[team][j + n] >= 0) {
 #pragma unroll
           for (int u = 0; u < TWO; ++u)
-            v[n][u] = part<T, W, TEAM>(p.rows + place[team][j + n] * row_bytes, i + u, me, p.cols);
+            v[n][u] = take(p.rows + place[team][j + n] * row_bytes, i + u, me, p.cols);
         }
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n)
@@ -1018,7 +1049,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) combine_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[u][e] += a[e];
       }
-      put<T, W, TEAM>(p.out + t * row_bytes, i + u, me, p.cols, Elem<T>::pack(sum[u]));
+      give(p.out + t * row_bytes, i + u, me, p.cols, Elem<T>::pack(sum[u]));
     }
   }
 }

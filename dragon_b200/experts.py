@@ -4,7 +4,7 @@ dgn_expert_* of include/dgn.h).
     indices, weights = route(logits, k, bias, mask)       # each token's experts
     p = plan(indices, num_experts)                        # where its rows go
     rows = dispatch(x, p)                                 # rows in the order of the experts
-    ...                                                   # expert e: rows[p.offsets[e]:p.offsets[e] + p.counts[e]]
+    ...                                                   # expert e: rows[p.offsets[e]:p.ends[e]]
     y = combine(outputs, p, weights, residual)            # the weighted sum back
 
     grad_outputs, grad_weights = combine_grad(grad_y, outputs, p, weights)
