@@ -967,13 +967,33 @@ __device__ __forceinline__ uint4 part_between(const char* row, int i, int me, in
   if (q) v = shift16(v, (int)q + left * (int)sizeof(T) > 16 ? from[1] : make_uint4(0, 0, 0, 0), q);
   return v;  // elements behind the last are the caller's to leave out
 }
+// Its counterpart, by whole warps: what a lane holds behind an aligned vector of the target goes to the next lane, so that
+// aligned vectors are written; only the ends of a warp's piece and of the row go by elements.
 template <typename T, int TEAM>
 __device__ __forceinline__ void put_between(char* row, int i, int me, int cols, uint4 v) {
   constexpr int E = Elem<T>::E;
-  const int c = (i * TEAM + me) * E;
+  typedef unsigned short U;
+  const int c = (i * TEAM + me) * E, left = cols - c, valid = min(left, E), lane = threadIdx.x & 31;
+  char* p = row + (size_t)c * sizeof(T);
+  const unsigned q = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);  // the same for all of a row
+  const uint4 before = make_uint4(__shfl_up_sync(kFull, v.x, 1), __shfl_up_sync(kFull, v.y, 1),
+                                  __shfl_up_sync(kFull, v.z, 1), __shfl_up_sync(kFull, v.w, 1));
+  if (left <= 0) return;
+  const int mine = (16 - (int)q) / (int)sizeof(T);  // elements in the aligned vector that p lies in
+  if (valid >= mine && (lane > 0 || q == 0)) {
+    *reinterpret_cast<uint4*>(p - q) = q ? shift16(before, v, 16 - q) : v;
+  } else {
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (c + e < cols) reinterpret_cast<unsigned short*>(row)[c + e] = reinterpret_cast<const unsigned short*>(&v)[e];
+    for (int e = 0; e < E; ++e) {
+      if (e >= mine && lane > 0) reinterpret_cast<U*>(p - 16)[e] = reinterpret_cast<const U*>(&before)[e];
+      if (e < min(mine, valid)) reinterpret_cast<U*>(p)[e] = reinterpret_cast<const U*>(&v)[e];
+    }
+  }
+  if (lane == 31 || left <= E) {  // nobody takes the rest
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e >= mine && e < valid) reinterpret_cast<U*>(p)[e] = reinterpret_cast<const U*>(&v)[e];
+  }
 }
 
 struct CombineParams {
@@ -1088,12 +1108,18 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid
     const char* row = p.rows + at * row_bytes;
     char* to = p.grad_rows + at * row_bytes;
     const int parts = (p.cols + 32 * E - 1) / (32 * E);
+    constexpr bool BETWEEN = W == 1 && sizeof(T) == 2;
     for (int i = 0; i < parts; i += AHEAD) {
       uint4 g[AHEAD], y[AHEAD];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {  // parts behind the last hold zeros and are not written
-        y[n] = part<T, W, 32>(row, i + n, lane, p.cols);
-        g[n] = part<T, W, 32>(grad, i + n, lane, p.cols);
+        if constexpr (BETWEEN) {
+          y[n] = part_between<T, 32>(row, i + n, lane, p.cols);
+          g[n] = part_between<T, 32>(grad, i + n, lane, p.cols);
+        } else {
+          y[n] = part<T, W, 32>(row, i + n, lane, p.cols);
+          g[n] = part<T, W, 32>(grad, i + n, lane, p.cols);
+        }
       }
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
@@ -1102,10 +1128,11 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const __grid
         Elem<T>::unpack(y[n], b);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          dot = fmaf(a[e], b[e], dot);
+          if (!BETWEEN || ((i + n) * 32 + lane) * E + e < p.cols) dot = fmaf(a[e], b[e], dot);
           a[e] *= w;
         }
-        put<T, W, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
+        if constexpr (BETWEEN) put_between<T, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
+        else put<T, W, 32>(to, i + n, lane, p.cols, Elem<T>::pack(a));
       }
     }
   }

@@ -290,7 +290,7 @@ def test_plan_passes_over_indices_that_do_not_exist(dgn_lib):
 
 
 MOVES = [(1, 1, 1, 16, 1), (3, 8, 256, 4096, 1), (5, 2, 4, 1, 4), (65, 3, 7, 769, 8), (200, 4, 16, 100, 128), (17, 32, 40, 1032, 1),
-         (300, 2, 9, 2048, 16), (2, 2, 2, 20000, 1)]
+         (300, 2, 9, 2048, 16), (2, 2, 2, 20000, 1), (40, 3, 8, 4099, 1), (9, 2, 3, 263, 8)]
 
 
 @pytest.mark.parametrize("tokens,k,num,cols,align", MOVES)
