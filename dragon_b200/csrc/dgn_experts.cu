@@ -635,20 +635,25 @@ __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_
     const float all = team_sum<L>((sum[0] + sum[1]) + (sum[2] + sum[3]));
     inv = all == 0.f ? 0.f : 1.f / all;
   }
+  // Renormalised weights do not change with a common factor of the scores, so their gradient only sees how the k weights'
+  // gradients differ: they are taken from the first one, and what the sum's small addend lets through is added apart.
+  // Without this one choice (whose weight is constant) would get the rounding of its own gradient.
+  const float common = p.renormalize ? __shfl_sync(kFull, ds[0], (threadIdx.x & 31) / L * L) : 0.f;
   float mine[Q], total = 0.f, dot = 0.f;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     mine[q] = logit[q] == -INFINITY ? 0.f : p.sigmoid ? 1.f / (1.f + expf(-logit[q])) : expf(logit[q] - top) * inv;
+    if (index[q] >= 0) ds[q] -= common;
     total += mine[q];
     dot += ds[q] * mine[q];
   }
   if (p.renormalize) {
     total = team_sum<L>(total) + kTiny;
-    const float along = team_sum<L>(dot) / total;
+    const float along = team_sum<L>(dot) / total, through = common * (kTiny / total);
     dot = 0.f;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      ds[q] = index[q] < 0 ? 0.f : (ds[q] - along) / total;
+      ds[q] = index[q] < 0 ? 0.f : (ds[q] - along + through) / total;
       dot += ds[q] * mine[q];
     }
   }

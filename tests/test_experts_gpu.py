@@ -222,6 +222,22 @@ def test_route_grad_of_odd_lists(dgn_lib):
 
 
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_grad_sees_differences_only(dgn_lib, scores):
+    """Renormalised weights of one choice are constant, and so are those under a gradient that all choices share."""
+    logits = normal(200, 24, seed=5)
+    one, _ = route(logits, 1, scores=scores)
+    grad = route_grad(normal(200, 1, seed=6), logits, one, scores=scores)
+    assert grad.abs().max() <= 1e-15  # 1e-20 over the score and its square, times a gradient of a few units
+    four, _ = route(logits, 4, scores=scores)
+    dw = normal(200, 4, seed=7)
+    a, b = (route_grad(w, logits, four, scores=scores) for w in (dw, dw + 64))
+    shifted = (dw + 64) - 64  # what the addition leaves of dw: differences of neighbours are exact
+    want, size = route_grad_reference(shifted, logits, four, scores, True, 1.0)
+    close(b, want, 100 * U * size, "shifted")
+    close(a, route_grad_reference(dw, logits, four, scores, True, 1.0)[0], 100 * U * size + 100 * U * size.amax(), "plain")
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_route_grad_against_differences(dgn_lib, scores, renormalize):
     logits, dw = normal(5, 48, seed=1), normal(5, 6, seed=2)
