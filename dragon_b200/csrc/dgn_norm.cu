@@ -229,25 +229,16 @@ __device__ __forceinline__ uint2 encode(const Pair* a, int code) {
   return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
+// (mean + eps)^(-1/2); 0 where the mean is infinite.
+__device__ __forceinline__ float inverse_root(float v) { return __frsqrt_rn(v); }
+
 // Codes of values h * w * rstd from u = h * w alone: with m the largest |u| of the group, code = rn(u * (L / m)) and
 // scale = m * rstd / L, so that rstd's rounding does not move a code.
-__device__ __forceinline__ float reciprocal(float m) {  // of normal numbers: the unit's estimate and one Newton step
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(m));
-  return fmaf(r, fmaf(-m, r, 1.f), r);
-}
-// (mean + eps)^(-1/2), likewise.
-__device__ __forceinline__ float inverse_root(float v) {
-  const float r = rsqrtf(v), half = 0.5f * r;
-  const float refined = fmaf(half, fmaf(-v * r, r, 1.f), r);
-  return v < __uint_as_float(0x7f800000u) ? refined : r;  // infinity: 0, not 0 * infinity
-}
 __device__ __forceinline__ float code_factor(float m, float rstd, float largest) {
   const float top = m * rstd;
   if (!(top < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);  // a NaN or an infinity: reads as NaN
   if (top < kSmallestAmax) return largest * rstd * (1.f / kSmallestAmax);
-  const float r = reciprocal(m), f = largest * r;
-  return fmaf(fmaf(-f, m, largest), r, f);  // the quotient, corrected by its remainder
+  return __fdiv_rn(largest, m);
 }
 __device__ __forceinline__ float code_scale(float m, float rstd, float inv_largest) {
   const float top = m * rstd;

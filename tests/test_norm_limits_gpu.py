@@ -1,0 +1,60 @@
+"""rms_norm at the ends of its ranges.
+
+u = 2^-24 is half a step of float32."""
+
+import pytest
+import torch
+
+from dragon_b200.normalization import rms_norm
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+CODES = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0, torch.float8_e5m2: 57344.0}
+DEV = "cuda:0"
+
+
+def normal(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g)).to(dtype).to(DEV)
+
+
+def grouped(t, width):
+    return t.reshape(t.shape[0], t.shape[1] // width, width)
+
+
+@pytest.mark.parametrize("out_dtype", list(CODES))
+@pytest.mark.parametrize("cols,group", [(64, 0), (64, 32), (96, 32), (33, 0)])
+def test_codes_of_products_whose_reciprocal_is_below_the_normal_numbers(dgn_lib, out_dtype, cols, group):
+    """hidden * weight between 2^126 and the largest float32: the largest code over it is an ordinary number all the same.
+    Groups whose largest value passes float32 (one in row 0, 3.9e38) report an infinity: their scale is NaN."""
+    x = normal(5, cols, seed=1, scale=1e17)
+    weight = torch.full((cols,), 1.2e38, device=DEV)
+    weight[::3] *= -0.5
+    x = x / x.abs().amax(1, keepdim=True) * 1.5
+    x[0], x[1] = x[0] * 0.6, x[1] * 1.8  # |h w| from 1.08e38 (2^126.3) to 3.2e38 at its largest
+    r = rms_norm(x, weight, out_dtype=out_dtype, group_size=group)
+    h = x.double()
+    y = h * (h.square().mean(1, keepdim=True) + 1e-6).rsqrt() * weight.double()
+    width, top = group or cols, CODES[out_dtype]
+    largest = grouped(y, width).abs().amax(2)
+    scale = torch.where(largest <= torch.finfo(torch.float32).max, largest / top, float("nan"))
+    fits = torch.isfinite(scale)
+    assert fits.float().mean() >= 0.8
+    assert torch.equal(torch.isnan(r.scale), torch.isnan(scale))
+    # The row's sum of at most 96 squares, its root, and three roundings.
+    assert ((r.scale.double() - scale).abs() <= 64 * U * scale)[fits].all()
+    wide = r.scale.double().repeat_interleave(width, 1)
+    half = 0.5 * wide if out_dtype == torch.int8 else torch.maximum(
+        torch.finfo(out_dtype).eps / 2 * y.abs(), torch.finfo(out_dtype).smallest_normal * torch.finfo(out_dtype).eps / 2 * wide)
+    off = (r.output.double() * wide - y).abs() - half - 72 * U * y.abs()
+    assert off[fits.repeat_interleave(width, 1)].max() <= 0
+
+
+def test_the_root_is_rounded_once(dgn_lib):
+    """One column: h^2 and its sum with eps are rounded, which the root halves, and the root: two times half a step."""
+    x = normal(4096, 1, seed=2) * torch.exp(normal(4096, 1, seed=3, scale=8.0))
+    x[0], x[1], x[2] = 0.0, 1e-30, 1.8e19
+    r = rms_norm(x, eps=1e-5)
+    want = (x.double().square()[:, 0] + torch.tensor(1e-5, dtype=torch.float32).double().item()).rsqrt()
+    assert ((r.rstd.double() - want).abs() <= 2.01 * U * want).all()
