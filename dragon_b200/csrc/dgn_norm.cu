@@ -233,13 +233,18 @@ __device__ __forceinline__ uint2 encode(const Pair* a, int code) {
 __device__ __forceinline__ float inverse_root(float v) { return __frsqrt_rn(v); }
 
 // Codes of values h * w * rstd from u = h * w alone: with m the largest |u| of the group, code = rn(u * (L / m)) and
-// scale = m * rstd / L, so that rstd's rounding does not move a code.
-__device__ __forceinline__ float code_factor(float m, float rstd, float largest) {
+// scale = m * rstd / L, so that rstd's rounding does not move a code.  L / m is kept as a quotient and its remainder's (the
+// double-length division of Dekker, 1971): of values of few bits u L / m often lies halfway between two codes, and one
+// float32 for L / m would leave that place by its rounding (27 codes of a million of bfloat16 rows and weights went to the
+// wrong neighbour; with both the product is rounded once).
+__device__ __forceinline__ float2 code_factor(float m, float rstd, float largest, float inv_largest) {
   const float top = m * rstd;
-  if (!(top < __uint_as_float(0x7f800000u))) return __uint_as_float(0x7fffffffu);  // a NaN or an infinity: reads as NaN
-  if (top < kSmallestAmax) return largest * rstd * (1.f / kSmallestAmax);
-  return __fdiv_rn(largest, m);
+  if (!(top < __uint_as_float(0x7f800000u))) return make_float2(__uint_as_float(0x7fffffffu), 0.f);  // NaN, infinity: NaN
+  if (top < kSmallestAmax) return make_float2(largest * rstd * (1.f / kSmallestAmax), 0.f);
+  const float f = __fdividef(0.25f * largest, 0.25f * m);  // a quarter: the call gives 0 for divisors above 2^126
+  return make_float2(f, fmaf(-f, m, largest) * (f * inv_largest));
 }
+__device__ __forceinline__ float times(float u, float2 f) { return fmaf(u, f.x, u * f.y); }
 __device__ __forceinline__ float code_scale(float m, float rstd, float inv_largest) {
   const float top = m * rstd;
   return top < __uint_as_float(0x7f800000u) ? fmaxf(top, kSmallestAmax) * inv_largest : __uint_as_float(0x7fffffffu);
@@ -255,7 +260,8 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
   constexpr int RU = !TEAM || !VEC ? 1 : NV == 1 ? 4 : NV == 2 ? 2 : 1;
   constexpr long long S = sizeof(T);
   __shared__ __align__(16) float slot[2][32];
-  __shared__ float chunk[VEC || !CODES ? 1 : 1024], factor[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
+  __shared__ float chunk[VEC || !CODES ? 1 : 1024];  // largest magnitude of 32 columns each
+  __shared__ float2 factor[VEC || !CODES ? 1 : 1024];
   const int team = TEAM ? TEAM : blockDim.x, me = threadIdx.x, cols = p.cols;
   const long long first = (long long)blockIdx.x * blockDim.y * RU + threadIdx.y;
   uint4 h[RU][NV], r[RU][NV];
@@ -365,7 +371,7 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
       for (int g = me; g < p.groups; g += team) {
         float m = 0.f;
         for (int k = g * of_group; k < min((g + 1) * of_group, chunks); ++k) m = Largest::of(m, chunk[threadIdx.y * 32 + k]);
-        factor[threadIdx.y * 32 + g] = code_factor(m, rstd[0], largest);
+        factor[threadIdx.y * 32 + g] = code_factor(m, rstd[0], largest, p.inv_largest);
         if (first < p.rows) p.scales[first * p.groups + g] = code_scale(m, rstd[0], p.inv_largest);
       }
       meet();
@@ -396,26 +402,26 @@ __global__ void __launch_bounds__(TEAM || (NV == 2 && W == Elem<T>::E) ? kThread
         if (c >= cols || row >= p.rows) continue;
         if (whole ? c == 0 : (c & ((1 << p.group_shift) - 1)) == 0)
           p.scales[row * p.groups + (whole ? 0 : c >> p.group_shift)] = code_scale(m, rstd[u], p.inv_largest);
-        const Pair f = twice(code_factor(m, rstd[u], largest));
+        const float2 f = code_factor(m, rstd[u], largest, p.inv_largest);
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) a[e] = a[e] * f;
+        for (int e = 0; e < E / 2; ++e) a[e] = fma2(a[e], twice(f.x), a[e] * twice(f.y));
         const uint2 codes = encode<E>(a, p.code);
         if (E == 8) *reinterpret_cast<uint2*>(out + c) = codes;
         else *reinterpret_cast<unsigned*>(out + c) = codes.x;
       } else {
-        const float all = code_factor(top[u], rstd[u], largest);
+        const float2 all = code_factor(top[u], rstd[u], largest, p.inv_largest);
         if (whole && me == 0 && i == 0 && row < p.rows) p.scales[row] = code_scale(top[u], rstd[u], p.inv_largest);
 #pragma unroll
         for (int e = 0; e < E; e += W) {
           const int c = column<T, W>(i, e, me, team);
           if (c >= cols || row >= p.rows) continue;
-          const float f = whole ? all : factor[threadIdx.y * 32 + (c >> p.group_shift)];
+          const float2 f = whole ? all : factor[threadIdx.y * 32 + (c >> p.group_shift)];
           const float2 v = a[e / 2].get();
           if (W == 2)
             *reinterpret_cast<unsigned short*>(out + c) =
-                (unsigned short)(encode1(v.x * f, p.code) | encode1(v.y * f, p.code) << 8);
+                (unsigned short)(encode1(times(v.x, f), p.code) | encode1(times(v.y, f), p.code) << 8);
           else
-            out[c] = (unsigned char)encode1((e & 1 ? v.y : v.x) * f, p.code);
+            out[c] = (unsigned char)encode1(times(e & 1 ? v.y : v.x, f), p.code);
         }
       }
     }

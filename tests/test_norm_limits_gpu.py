@@ -58,3 +58,19 @@ def test_the_root_is_rounded_once(dgn_lib):
     r = rms_norm(x, eps=1e-5)
     want = (x.double().square()[:, 0] + torch.tensor(1e-5, dtype=torch.float32).double().item()).rsqrt()
     assert ((r.rstd.double() - want).abs() <= 2.01 * U * want).all()
+
+
+@pytest.mark.parametrize("out_dtype", list(CODES))
+@pytest.mark.parametrize("cols", [512, 514, 515, 4096])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_codes_are_the_nearest_ones_between_neighbours_too(dgn_lib, out_dtype, cols, group):
+    """Products u of bfloat16 rows and weights have 16 bits, so that u L / m is often halfway between two codes and
+    otherwise at least 2^-41 of itself away from where float32 rounds: whoever rounds the quotient once gets these codes."""
+    x, weight = normal(256, cols, seed=4, dtype=torch.bfloat16), normal(cols, seed=5, dtype=torch.bfloat16)
+    r = rms_norm(x, weight, out_dtype=out_dtype, group_size=group)
+    u, width = x.double() * weight.double(), group or cols
+    groups = -(-cols // width)
+    m = torch.nn.functional.pad(u, (0, groups * width - cols)).view(256, groups, width).abs().amax(2)
+    q = (u * CODES[out_dtype] / m.repeat_interleave(width, 1)[:, :cols]).float()
+    want = (q.round() if out_dtype == torch.int8 else q).to(out_dtype)
+    assert torch.equal(r.output.view(torch.uint8), want.view(torch.uint8))
