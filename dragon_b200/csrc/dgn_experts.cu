@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
       word[i] = x[i] > -INFINITY ? (__float_as_uint(step) - 0x4affffffu) << p.bits | (low - e) : 0;
     }
     // The place's own rounding is below two steps for each of two words; keys are off by half the slack and their rounding.
-    need = 5 + (unsigned)fminf((slack + 0x1p-22f * fmaxf(fabsf(most), fabsf(base))) * scale, 1e6f);
+    // In a row whose keys differ by less than that no two words are far enough apart, at any number of steps.
+    need = 5 + (unsigned)fminf((slack + 0x1p-22f * fmaxf(fabsf(most), fabsf(base))) * scale, 0x1p30f);
   }
   unsigned last = kWrap;
   const auto next_word = [&](int j) {
