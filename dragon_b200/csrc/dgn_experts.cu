@@ -392,11 +392,18 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
   }
 
   if (p.groups > 1) {
-    float worst = INFINITY, next = -INFINITY;  // the values on either side of the border
+    // On either side of the border: the least that a kept group may be worth, and the most that another one may be.  A value
+    // is off by what its keys are, each by half the slack and its rounding, and by its own rounding.  The keys' magnitudes
+    // count, not the sum's: keys of +8 and -8 add up to nothing but their roundings.
+    const bool rounded = p.bias || p.best == 2;  // logits alone are compared as they are
+    float worst = INFINITY, next = -INFINITY;
+    const auto error_of = [&](float a, float b) {
+      return rounded ? slack + 0x1p-22f * (fabsf(a) + (p.best == 2 && b > -INFINITY ? fabsf(b) : 0.f)) : 0.f;
+    };
     if (VEC && p.group_lanes) {
       // A group is p.group_lanes neighbouring lanes' vectors: its value is made and compared in registers.
       constexpr int V = 16 / (int)sizeof(T), C = VEC ? N / V : 1;
-      float value[C];
+      float value[C], error[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float a = -INFINITY, b = -INFINITY;
@@ -412,6 +419,7 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
           a = fmaxf(a, oa);
         }
         value[c] = p.best == 2 && b > -INFINITY ? a + b : a;
+        error[c] = error_of(a, b);
       }
       int rank[C];
 #pragma unroll
@@ -428,9 +436,9 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
       for (int c = 0; c < C; ++c) {
         const bool there = expert_of<T, L, VEC>(c * V, lane) < experts;
         if (rank[c] < p.keep) {
-          if (there) worst = fminf(worst, value[c]);
+          if (there && value[c] > -INFINITY) worst = fminf(worst, value[c] - error[c]);
         } else {
-          next = fmaxf(next, value[c]);
+          if (value[c] > -INFINITY) next = fmaxf(next, value[c] + error[c]);
 #pragma unroll
           for (int i = 0; i < V; ++i) x[c * V + i] = -INFINITY;
         }
@@ -446,7 +454,11 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
         values[e + (e * p.magic >> 20)] = v;  // a word between the groups keeps them in different banks
       }
       __syncwarp();
-      for (int g = lane; g < p.groups; g += L) {
+      float error[kMaxGroups / L];  // of the groups lane, lane + L, ...
+#pragma unroll
+      for (int n = 0; n < kMaxGroups / L; ++n) {
+        const int g = n * L + lane;
+        if (g >= p.groups) break;
         float a = -INFINITY, b = -INFINITY;
 #pragma unroll 8
         for (int i = 0; i < width; ++i) {
@@ -455,18 +467,22 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
           a = fmaxf(a, v);
         }
         group_value[g] = p.best == 2 && b > -INFINITY ? a + b : a;
+        error[n] = error_of(a, b);
       }
       __syncwarp();
       unsigned kept = 0;
-      for (int g = lane; g < p.groups; g += L) {
+#pragma unroll
+      for (int n = 0; n < kMaxGroups / L; ++n) {
+        const int g = n * L + lane;
+        if (g >= p.groups) break;
         const float v = group_value[g];
         int rank = 0;
         for (int o = 0; o < p.groups; ++o) rank += group_value[o] > v || (group_value[o] == v && o < g);
         if (rank < p.keep) {
           kept |= 1u << g;
-          worst = fminf(worst, v);
-        } else {
-          next = fmaxf(next, v);
+          if (v > -INFINITY) worst = fminf(worst, v - error[n]);
+        } else if (v > -INFINITY) {
+          next = fmaxf(next, v + error[n]);
         }
       }
 #pragma unroll
@@ -477,9 +493,7 @@ __global__ void __launch_bounds__(kRouteThreads, N <= 16 ? 8 : 5) route_kernel(c
     }
     worst = -team_max<L>(-worst);
     next = team_max<L>(next);
-    // Logits alone are compared as they are; sums and scores have to be further apart than they may be off.
-    if ((p.bias || p.best == 2) && p.keep < p.groups && next > -INFINITY)
-      odd |= !(worst - next > 2.f * slack + 0x1p-22f * (fabsf(worst) + fabsf(next)));
+    if (rounded && p.keep < p.groups && next > -INFINITY) odd |= !(worst > next);
   }
 
   // Words: the upper bits of the key's order, or of its place between the largest and the smallest key.

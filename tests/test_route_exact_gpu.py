@@ -103,3 +103,39 @@ def test_two_experts_far_apart_in_steps(dgn_lib, scores):
         logits = torch.log(score) - torch.log1p(-score)
     logits = logits + 1e-7 * torch.randn(4000, 2, generator=g, dtype=torch.float64)
     check(logits.float(), bias, 1, scores)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("width", [32, 24])  # a power of two of vectors, and groups that go through shared memory
+@pytest.mark.parametrize("offset", [0.5, 4.0, 8.0, 32.0, 512.0])
+@pytest.mark.parametrize("groups", [2, 4])
+def test_groups_whose_keys_cancel(dgn_lib, scores, width, offset, groups):
+    """The two best of each group are one of bias +offset and one of -offset: their sum is small, its rounding is not."""
+    tokens, g = 4000, generator(int(offset * 2) + groups)
+    logits = torch.randn(tokens, 1, width, generator=g).repeat(1, groups, 1)
+    logits += torch.randn(tokens, groups, width, generator=g) * 10 ** (-7 + 3 * torch.rand(tokens, 1, 1, generator=g))
+    bias = torch.full((groups, width), -offset)
+    bias[:, 3] = offset
+    check(logits.view(tokens, -1), bias.view(-1), 2, scores, groups=groups, keep=1, best=2)
+    check(logits.view(tokens, -1), bias.view(-1), 4, scores, groups=groups, keep=max(1, groups - 1), best=2)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("best", [1, 2])
+def test_groups_of_nearly_equal_scores(dgn_lib, scores, best):
+    """Without a bias, and with one of nothing: sums of scores, and logits that are compared as they are."""
+    tokens, groups, width, g = 4000, 4, 16, generator(9)
+    logits = torch.randn(tokens, 1, width, generator=g).repeat(1, groups, 1)
+    logits += torch.randn(tokens, groups, width, generator=g) * 10 ** (-8 + 4 * torch.rand(tokens, 1, 1, generator=g))
+    check(logits.view(tokens, -1), torch.zeros(groups * width), 3, scores, groups=groups, keep=2, best=best)
+
+
+def test_experts_closed_by_a_low_bias(dgn_lib):
+    """A bias of -1e9 closes an expert as -inf does, in groups that have open ones and in groups that have none."""
+    tokens, groups, width, g = 500, 4, 8, generator(10)
+    logits, bias = torch.randn(tokens, groups * width, generator=g), 0.1 * torch.randn(groups * width, generator=g)
+    bias[1:8] = -1e9  # one expert is open in the first group, none in the second
+    bias[8:16] = -1e9
+    for scores in ("softmax", "sigmoid"):
+        for best in (1, 2):
+            check(logits, bias, 4, scores, groups=groups, keep=2, best=best)
