@@ -7,7 +7,7 @@ of each other without being equal are left out; there is about one in 1e7."""
 import pytest
 import torch
 
-from dragon_b200.experts import route
+from dragon_b200.experts import route, route_grad
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,34 @@ def test_experts_closed_by_a_low_bias(dgn_lib):
     for scores in ("softmax", "sigmoid"):
         for best in (1, 2):
             check(logits, bias, 4, scores, groups=groups, keep=2, best=best)
+
+
+U = 2.0 ** -24  # half a step of float32
+
+
+@pytest.mark.parametrize("num", [8, 61, 256, 600])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_gradients_of_small_scores_have_the_bits_of_float32(dgn_lib, num, scores):
+    """One choice and no renormalisation: dl_e = -dw s_c s_e for the softmax's other experts, dw s (1 - s) for the sigmoid.
+
+    Distances up to 85 from the row's largest logit, which is 0, so that the exponentials' arguments are exact: 4 u each (two
+    steps of expf).  Their sum: 4 u and 15 additions after one another, a reciprocal: 20 u, which both scores have.  The
+    exponential of e 4 u, four products.  48 u in all."""
+    tokens, g = 64, generator(num)
+    logits = -85 * torch.rand(tokens, num, generator=g)
+    chosen = torch.randint(0, num, (tokens, 1), generator=g)
+    logits.scatter_(1, chosen, 0.0)
+    dw = torch.randn(tokens, 1, generator=g)
+    if scores == "sigmoid":
+        logits.scatter_(1, chosen, 170 * torch.rand(tokens, 1, generator=g) - 85)
+    got = route_grad(dw.to(DEV), logits.to(DEV), chosen.int().to(DEV), scores=scores, renormalize=False).cpu().double()
+    l = logits.double()
+    if scores == "sigmoid":
+        want = torch.zeros_like(l).scatter_(1, chosen, dw.double() * (torch.sigmoid(l) * torch.sigmoid(-l)).gather(1, chosen))
+        # One exponential of the logit itself, whose argument is exact, a sum, a quotient, three products.
+        assert ((got - want).abs() <= 16 * U * want.abs() + 1e-44).all()
+        return
+    s = torch.softmax(l, 1)
+    want = -dw.double() * s.gather(1, chosen) * s
+    others = torch.ones_like(l, dtype=torch.bool).scatter_(1, chosen, False)
+    assert ((got - want).abs() <= 48 * U * want.abs() + 1e-44)[others].all()
