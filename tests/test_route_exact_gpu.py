@@ -170,3 +170,13 @@ def test_gradients_of_small_scores_have_the_bits_of_float32(dgn_lib, num, scores
     want = -dw.double() * s.gather(1, chosen) * s
     others = torch.ones_like(l, dtype=torch.bool).scatter_(1, chosen, False)
     assert ((got - want).abs() <= 48 * U * want.abs() + 1e-44)[others].all()
+
+
+@pytest.mark.parametrize("num", [8, 61, 256, 600])
+def test_weights_as_they_are_have_the_bits_of_float32(dgn_lib, num):
+    """Without renormalisation a weight is its score: an exponential (4 u and its argument's rounding, differences below 12)
+    over a sum of positive ones (4 u + 12 u, 22 additions), two roundings."""
+    logits = 2 * torch.randn(2000, num, generator=generator(num))
+    indices, weights = route(logits.to(DEV), 4, renormalize=False)
+    want = torch.softmax(logits.double(), 1).gather(1, indices.cpu().long())
+    assert ((weights.cpu().double() - want).abs() <= 60 * U * want).all()
