@@ -36,11 +36,14 @@ class OnDevice {
   cudaError_t err_;
 };
 
-// Lets `fn` be launched with `smem` bytes of dynamic shared memory.  Without this the
-// dynamic and the static part together may take 48 KiB; static parts here are below 8.
+// Lets `fn` be launched with `smem` bytes of dynamic shared memory.  Without this the dynamic and the static part together
+// may take 48 KiB; static parts of the kernels that have a dynamic one are below 1 KiB.  The limit belongs to the function
+// and not to the launch: it is the same for every call, so that no thread lowers it between another's call and its launch.
+constexpr int kMostDynamicShared = 224 << 10;  // of the 227 KiB that a block can have
+
 inline int allow_shared(const void* fn, size_t smem) {
   if (smem <= (40 << 10)) return DGN_OK;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicShared);
   if (e == cudaSuccess) return DGN_OK;
   cudaGetLastError();
   return report_error(DGN_ERR_CUDA, cudaGetErrorString(e));

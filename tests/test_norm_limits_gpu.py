@@ -2,10 +2,13 @@
 
 u = 2^-24 is half a step of float32."""
 
+import threading
+
 import pytest
 import torch
 
-from dragon_b200.normalization import rms_norm
+from dragon_b200 import _C
+from dragon_b200.normalization import rms_norm, rms_norm_grad
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +77,32 @@ def test_codes_are_the_nearest_ones_between_neighbours_too(dgn_lib, out_dtype, c
     q = (u * CODES[out_dtype] / m.repeat_interleave(width, 1)[:, :cols]).float()
     want = (q.round() if out_dtype == torch.int8 else q).to(out_dtype)
     assert torch.equal(r.output.view(torch.uint8), want.view(torch.uint8))
+
+
+def test_two_threads_with_kernels_of_different_size(dgn_lib):
+    """Callers of the C-ABI on threads of their own: the same kernel with more and with less shared memory at the same time."""
+    failed, outputs = [], {}
+
+    def work(cols):
+        dy, h, gh = (normal(64, cols, seed=s, dtype=torch.bfloat16) for s in (1, 2, 3))
+        rstd, out = rms_norm(h).rstd, torch.empty_like(h)
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for _ in range(3000):
+            rc = dgn_lib.dgn_rms_norm_grad(dy.data_ptr(), cols, gh.data_ptr(), cols, h.data_ptr(), cols, None, _C.F32,
+                                           rstd.data_ptr(), out.data_ptr(), None, None, 0, 64, cols, _C.BF16, 0,
+                                           stream.cuda_stream)
+            if rc != _C.OK:
+                failed.append((cols, rc))
+                break
+        stream.synchronize()
+        outputs[cols] = (out, rms_norm_grad(dy, h, rstd, None, gh)[0])
+
+    threads = [threading.Thread(target=work, args=(cols,)) for cols in (4096, 2560, 2048)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    torch.cuda.synchronize()
+    assert len(outputs) == 3 and all(torch.equal(a, b) for a, b in outputs.values())
