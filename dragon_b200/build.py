@@ -6,10 +6,12 @@
 * ``dragon_b200/lib/libdragon_collective.so`` -- the C++ operator layer over it
   (built when its sources are present)
 * ``dragon_b200/lib/dgn_torch.so`` -- the torch calls of the norm and expert
-  operators, an extension module (built against the installed torch)
+  operators, an extension module (built against the installed torch; left out
+  where there is none)
 
-Objects are rebuilt only when a source or header is newer.  nvcc cross-compiles
-without a GPU, so this runs on any machine with the CUDA toolkit.
+Objects are rebuilt only when a source or header is newer, the extension module
+also under another Python or torch.  nvcc cross-compiles without a GPU, so this
+runs on any machine with the CUDA toolkit.
 """
 
 import concurrent.futures
@@ -59,15 +61,21 @@ def _headers():
     return hdrs
 
 
-def _torch_object(obj, src):
-    """Command that compiles the extension module's source, and what it depends on."""
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+def _torch_object(obj, src, torch_dir):
+    """Command that compiles the extension module's source, and a file that is
+    newer than the object under another Python or torch than it was built for."""
     inc = os.path.join(torch_dir, "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-c", src, "-o", obj]
     for path in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), cuda):
         cmd += ["-isystem", path]
-    return cmd + ["-isystem", sysconfig.get_paths()["include"]], os.path.join(torch_dir, "version.py")
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        versions = "\n".join([sys.version, sysconfig.get_paths()["include"], torch_dir, f.read()])
+    stamp = os.path.splitext(obj)[0] + ".versions"
+    if not os.path.exists(stamp) or open(stamp).read() != versions:
+        with open(stamp, "w") as f:
+            f.write(versions)
+    return cmd + ["-isystem", sysconfig.get_paths()["include"]], stamp
 
 
 def build(verbose=False, extra_flags=()):
@@ -89,8 +97,11 @@ def build(verbose=False, extra_flags=()):
             cmd = [nvcc] + NVCC_FLAGS + list(extra_flags) + ["-c", src, "-o", obj]
             jobs.append((obj, cmd, [src] + hdrs))
     torch_src, torch_obj = os.path.join(CSRC, "dgn_torch.cc"), os.path.join(OBJ, "dgn_torch.o")
-    torch_cmd, torch_version = _torch_object(torch_obj, torch_src)
-    jobs.append((torch_obj, torch_cmd, [torch_src, torch_version, hdrs[0]]))
+    torch_spec = importlib.util.find_spec("torch")
+    if torch_spec is not None:
+        torch_dir = os.path.dirname(torch_spec.origin)
+        torch_cmd, stamp = _torch_object(torch_obj, torch_src, torch_dir)
+        jobs.append((torch_obj, torch_cmd, [torch_src, stamp, hdrs[0]]))
     stale = [(o, c) for o, c, deps in jobs if _newer(o, deps)]
     if stale:
         workers = min(len(stale), os.cpu_count() or 4)
@@ -117,9 +128,11 @@ def build(verbose=False, extra_flags=()):
 
     # The extension module; torch's own libraries are loaded by the time it is imported.
     ext = os.path.join(LIB, "dgn_torch.so")
-    if _newer(ext, [torch_obj, lib]):
-        _run(["g++", "-shared", "-o", ext, torch_obj, "-L", os.path.join(os.path.dirname(torch_version), "lib"), "-ltorch",
-              "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-L", LIB, "-ldgn", "-Wl,-rpath,$ORIGIN"])
+    if torch_spec is None:
+        print("torch is not installed: dgn_torch.so, the Python calls of the norm and expert operators, is left out")
+    elif _newer(ext, [torch_obj, lib]):
+        _run(["g++", "-shared", "-o", ext, torch_obj, "-L", os.path.join(torch_dir, "lib"), "-ltorch", "-ltorch_cpu",
+              "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-L", LIB, "-ldgn", "-Wl,-rpath,$ORIGIN"])
     return lib
 
 
