@@ -31,6 +31,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, out_dtype=None, group_size
     torch.float8_e5m2: then output * scale stands for the value, with one float32
     scale per row and `group_size` columns (32, 64, 128, or 0 for the row).
 
+    The sum of a row's squares is held in float32: rows where it passes 3.4e38
+    (4096 columns of 2.9e17 each) come out as zeros, with rstd 0.
+
     Returns RMSNorm(output, hidden, rstd, scale)."""
     if stream is not None:
         with _enter_stream(stream, x.device):

@@ -368,9 +368,10 @@ int dgn_allreduce_static_status(int clear);
  * hidden is x itself and not written), rstd = 1/sqrt(mean(hidden^2) + eps),
  * out = hidden * rstd * weight.  dtype: DGN_F16, DGN_BF16, DGN_F32; 1..32768
  * columns.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
- * be the residual's own memory, with the same stride.  The sum of squares is
- * held in float32: a row whose mean square passes 3.4e38 comes out as zeros.  With a code, out holds 8-bit values instead and scales one
- * float32 per row and group of `group` columns (32, 64, 128, or 0: the row):
+ * be the residual's own memory, with the same stride.  The sum of a row's squares
+ * is held in float32: rows where it passes 3.4e38 (4096 columns of 2.9e17 each)
+ * come out as zeros, with rstd 0.  With a code, out holds 8-bit values instead and
+ * scales one float32 per row and group of `group` columns (32, 64, 128, or 0: the row):
  * value = code * scale, scale = largest magnitude / largest code (127, 448,
  * 57344), groups below 2^-40 taking that bound's scale; a group with a NaN or an
  * infinity has scale NaN.  out, scales [rows, groups] and rstd are contiguous. */

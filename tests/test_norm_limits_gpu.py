@@ -106,3 +106,19 @@ def test_two_threads_with_kernels_of_different_size(dgn_lib):
     assert not failed
     torch.cuda.synchronize()
     assert len(outputs) == 3 and all(torch.equal(a, b) for a, b in outputs.values())
+
+
+@pytest.mark.parametrize("cols,dtype", [(64, torch.float32), (4096, torch.float32), (4096, torch.bfloat16), (1025, torch.float32),
+                                        (32768, torch.float32)])
+def test_the_sum_of_squares_has_the_range_of_float32(dgn_lib, cols, dtype):
+    """Whatever the order of the additions: right below 2^128, zeros from there on.
+
+    At most 74 additions follow one another (64 in a thread, 10 across threads), each half a step, and with the products'
+    own the sum is off by 80 u, its root by half of that and a few roundings: 45 u; the output adds four more and its type's."""
+    edge = (2.0 ** 128 / cols) ** 0.5
+    x = torch.stack([torch.full((cols,), f * edge) for f in (0.98, 0.9, 1.02, 10.0)]).to(dtype).to(DEV)
+    r = rms_norm(x)
+    assert ((r.output[:2].double() - 1).abs() <= 49 * U + torch.finfo(dtype).eps / 2).all()
+    want = x[:2, 0].double().reciprocal()
+    assert ((r.rstd[:2].double() - want).abs() <= 45 * U * want).all()
+    assert (r.output[2:] == 0).all() and (r.rstd[2:] == 0).all()
