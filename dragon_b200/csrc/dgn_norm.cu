@@ -793,7 +793,8 @@ extern "C" int dgn_rms_norm(const void* x, int64_t x_stride, const void* residua
                             int dtype, int device, void* stream) {
   int rc = check_matrix(rows, cols, dtype);
   if (rc != DGN_OK) return rc;
-  if (!(eps > 0.f) || isinf(eps)) return report_error(DGN_ERR_ARG, "eps must be a positive number");
+  // Not below the normal numbers: rstd of a row of zeros times the inverse of the smallest scale stays finite.
+  if (!(eps >= 0x1p-126f) || isinf(eps)) return report_error(DGN_ERR_ARG, "eps must be a positive number, 2^-126 at least");
   if (code < DGN_CODE_NONE || code > DGN_CODE_E5M2) return report_error(DGN_ERR_ARG, "unknown 8-bit code");
   if (group != 0 && group != 32 && group != 64 && group != 128)
     return report_error(DGN_ERR_ARG, "a scale covers 32, 64 or 128 columns, or the row (0)");

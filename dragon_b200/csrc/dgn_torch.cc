@@ -131,7 +131,7 @@ std::tuple<Tensor, Tensor, Tensor, MaybeTensor> rms_norm(const Tensor& x, const 
                                                           bool in_place) {
   check_norm_input(x, "x");
   const Rows r = rows_of(x, "x");
-  if (!(eps > 0) || eps > 3.4e38 || !((float)eps > 0.f)) value_error("<eps> must be a positive number");
+  if (!(eps >= 0x1p-126) || eps > 3.4e38) value_error("<eps> must be a positive number, 2^-126 at least");
   if (group != 0 && group != 32 && group != 64 && group != 128)
     value_error("<group_size> must be one of (0, 32, 64, 128), got " + std::to_string(group));
   const ScalarType type = x.scalar_type(), out = out_type.value_or(type);

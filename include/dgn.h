@@ -367,7 +367,7 @@ int dgn_allreduce_static_status(int clear);
  * dgn_rms_norm: hidden = x + residual (rounded to `dtype`; without a residual
  * hidden is x itself and not written), rstd = 1/sqrt(mean(hidden^2) + eps),
  * out = hidden * rstd * weight.  dtype: DGN_F16, DGN_BF16, DGN_F32; 1..32768
- * columns.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
+ * columns; eps 2^-126 at least.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
  * be the residual's own memory, with the same stride.  The sum of a row's squares
  * is held in float32: rows where it passes 3.4e38 (4096 columns of 2.9e17 each)
  * come out as zeros, with rstd 0.  With a code, out holds 8-bit values instead and

@@ -122,3 +122,14 @@ def test_the_sum_of_squares_has_the_range_of_float32(dgn_lib, cols, dtype):
     want = x[:2, 0].double().reciprocal()
     assert ((r.rstd[:2].double() - want).abs() <= 45 * U * want).all()
     assert (r.output[2:] == 0).all() and (r.rstd[2:] == 0).all()
+
+
+@pytest.mark.parametrize("out_dtype", list(CODES))
+@pytest.mark.parametrize("cols", [64, 65])
+def test_the_smallest_eps(dgn_lib, out_dtype, cols):
+    """Rows of zeros stay zeros, and the smallest scale is theirs; a smaller eps is refused."""
+    r = rms_norm(torch.zeros(3, cols, device=DEV), eps=2.0 ** -126, out_dtype=out_dtype)
+    assert (r.output.float() == 0).all() and (r.scale.double() * CODES[out_dtype] * 2.0 ** 40 - 1).abs().max() <= U
+    for eps in (1e-45, 2.0 ** -127):
+        with pytest.raises(ValueError, match="eps"):
+            rms_norm(torch.zeros(3, cols, device=DEV), eps=eps, out_dtype=out_dtype)
