@@ -61,6 +61,11 @@ const void* address(const MaybeTensor& t) { return t ? t->const_data_ptr() : nul
 void check_cuda(const Tensor& t, const char* name) {
   if (!t.is_cuda()) value_error(std::string("<") + name + "> must be a CUDA tensor (got " + t.device().str() + ")");
 }
+// Views that stand for other values than their memory holds (x.conj(), the imaginary part of one).
+void check_plain(const Tensor& t, const char* name) {
+  if (t.is_conj() || t.is_neg())
+    value_error(std::string("<") + name + "> is a conjugate or negative view: resolve_conj() and resolve_neg() make its values");
+}
 void check_device(const Tensor& t, const Tensor& like, const char* name) {
   if (t.device() != like.device())
     value_error(std::string("<") + name + "> must live on " + like.device().str() + " (got " + t.device().str() + ")");
@@ -72,6 +77,7 @@ void check_shape(const Tensor& t, at::IntArrayRef shape, const char* name) {
 // A contiguous tensor of one device, shape and type.
 void check_exactly(const Tensor& t, const Tensor& like, at::IntArrayRef shape, ScalarType type, const char* name) {
   if (t.scalar_type() != type) unsupported(name, t.scalar_type());
+  check_plain(t, name);
   check_device(t, like, name);
   check_shape(t, shape, name);
   if (!t.is_contiguous()) value_error(std::string("<") + name + "> must be contiguous");
@@ -84,6 +90,7 @@ struct Rows {
 Rows rows_of(const Tensor& t, const char* name) {
   const std::string n = std::string("<") + name + ">";
   if (t.dim() == 0) value_error(n + " needs at least one dimension");
+  check_plain(t, name);
   const int64_t cols = t.size(-1);
   if (t.is_contiguous()) return {cols ? t.numel() / cols : 0, cols, cols};
   if (t.stride(-1) != 1 && cols > 1) value_error("the last dimension of " + n + " must be contiguous");
@@ -120,6 +127,7 @@ void check_like(const Tensor& t, const Tensor& x, const char* name) {
 void check_weight(const Tensor& weight, const Tensor& x, int64_t cols) {
   if (weight.scalar_type() != x.scalar_type() && weight.scalar_type() != ScalarType::Float)
     type_error("<weight> must be float32 or " + name_of(x.scalar_type()) + ", got " + name_of(weight.scalar_type()));
+  check_plain(weight, "weight");
   check_device(weight, x, "weight");
   if (weight.dim() != 1 || weight.size(0) != cols || !weight.is_contiguous())
     value_error("<weight> must be a contiguous vector of " + std::to_string(cols) + " elements");
