@@ -988,7 +988,8 @@ __device__ __forceinline__ uint4 part_between(const char* row, int i, int me, in
   const unsigned q = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15);
   const uint4* from = reinterpret_cast<const uint4*>(p - q);
   uint4 v = from[0];
-  if (q) v = shift16(v, (int)q + left * (int)sizeof(T) > 16 ? from[1] : make_uint4(0, 0, 0, 0), q);
+  const int here = (16 - (int)q) / (int)sizeof(T);  // elements in the first vector; compared as such, bytes may pass 31 bits
+  if (q) v = shift16(v, left > here ? from[1] : make_uint4(0, 0, 0, 0), q);
   return v;  // elements behind the last are the caller's to leave out
 }
 // Its counterpart, by whole warps: what a lane holds behind an aligned vector of the target goes to the next lane, so that

@@ -33,3 +33,20 @@ def test_views_that_stand_for_other_values_are_refused(dgn_lib):
                  lambda: route(x, 1, bias=vector)):
         with pytest.raises(ValueError, match="view"):
             call()
+
+
+def test_the_longest_odd_rows(dgn_lib):
+    """Rows whose bytes pass 31 bits with the offset of an unaligned start."""
+    cols = (1 << 30) - 1
+    p = plan(torch.arange(2, dtype=torch.int32, device=DEV)[:, None].contiguous(), 2)
+    rows = torch.empty(2, cols, dtype=torch.float16, device=DEV)
+    rows[0], rows[1] = 1.0, 2.0
+    rows[:, :64] = normal(2, 64, seed=1, dtype=torch.float16)
+    rows[:, -64:] = normal(2, 64, seed=2, dtype=torch.float16)
+    assert torch.equal(combine(rows, p), rows)
+    del rows
+    one, row = plan(torch.zeros(1, 1, dtype=torch.int32, device=DEV), 1), torch.ones(1, cols + 1, dtype=torch.float16, device=DEV)
+    residual = torch.ones(1, cols + 9, dtype=torch.float16, device=DEV)
+    residual[:, :64] = 3.0
+    cut = residual[:, 1:cols + 2]
+    assert torch.equal(combine(row, one, residual=cut), cut + 1)
