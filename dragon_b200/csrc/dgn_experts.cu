@@ -1273,7 +1273,7 @@ int check_route(int64_t tokens, int64_t stride, int experts, int k, int score, i
 }
 
 int check_move(int64_t tokens, int k, int64_t capacity, int64_t row) {
-  if (tokens < 0 || k < 1 || k > kMaxChoices || tokens * k > INT32_MAX)
+  if (tokens < 0 || tokens > INT32_MAX || k < 1 || k > kMaxChoices || tokens * k > INT32_MAX)
     return report_error(DGN_ERR_ARG, "a token has 1..32 choices, a call fewer than 2^31");
   if (capacity < 0 || capacity > INT32_MAX) return report_error(DGN_ERR_ARG, "capacity must be 0..2^31-1 rows");
   if (row < 1 || row > kMaxRow) return report_error(DGN_ERR_ARG, "rows must not be empty or pass 2^30 elements or bytes");
