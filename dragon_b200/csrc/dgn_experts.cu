@@ -17,9 +17,8 @@ namespace {
 
 using namespace dgn;
 
-constexpr int kMaxExperts = 1024;
-constexpr int kMaxChoices = 32;  // one lane of a warp for each
-constexpr int kMaxGroups = 32;
+constexpr int kMaxExperts = DGN_MAX_EXPERTS, kMaxGroups = DGN_MAX_GROUPS;
+constexpr int kMaxChoices = DGN_MAX_CHOICES;  // one lane of a warp for each
 constexpr int64_t kMaxRow = 1 << 30;  // so that a column plus a block's width stays a 32-bit number
 constexpr float kTiny = 1e-20f;  // keeps the sum that weights are divided by from zero
 constexpr unsigned kFull = 0xffffffffu;

@@ -24,8 +24,6 @@ typedef std::optional<Tensor> MaybeTensor;
 
 namespace {
 
-constexpr int64_t kMaxExperts = 1024, kMaxChoices = 32, kMaxGroups = 32;
-
 std::string name_of(ScalarType t) { return py::str(py::cast(t)).cast<std::string>(); }
 std::string name_of(at::IntArrayRef shape) {
   std::string s = "(";
@@ -215,13 +213,14 @@ std::tuple<Tensor, MaybeTensor> rms_norm_grad(const Tensor& grad_output, const T
 // ---- experts ---------------------------------------------------------------------------
 
 void check_experts(int64_t experts) {
-  if (experts < 1 || experts > kMaxExperts)
-    value_error("there must be 1 to 1024 experts, got " + std::to_string(experts));
+  if (experts < 1 || experts > DGN_MAX_EXPERTS)
+    value_error("there must be 1 to " + std::to_string(DGN_MAX_EXPERTS) + " experts, got " + std::to_string(experts));
 }
 void check_choice(int64_t k, int64_t experts) {
   check_experts(experts);
-  if (k < 1 || k > kMaxChoices || k > experts)
-    value_error("<k> must be 1 to 32 and at most the number of experts, got " + std::to_string(k));
+  if (k < 1 || k > DGN_MAX_CHOICES || k > experts)
+    value_error("<k> must be 1 to " + std::to_string(DGN_MAX_CHOICES) + " and at most the number of experts, got " +
+                std::to_string(k));
 }
 const float* floats(const MaybeTensor& t) { return t ? t->const_data_ptr<float>() : nullptr; }
 
@@ -229,8 +228,8 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const MaybeTen
                                  int score, int64_t groups, int64_t keep, int64_t best, bool renormalize, double scale) {
   const int64_t stride = matrix(logits, "logits"), tokens = logits.size(0), experts = logits.size(1);
   check_choice(k, experts);
-  if (groups < 1 || groups > kMaxGroups || experts % groups)
-    value_error("<groups> must be 1 to 32 and divide the number of experts");
+  if (groups < 1 || groups > DGN_MAX_GROUPS || experts % groups)
+    value_error("<groups> must be 1 to " + std::to_string(DGN_MAX_GROUPS) + " and divide the number of experts");
   if (keep < 1 || keep > groups) value_error("<keep_groups> must be 1 to <groups>, got " + std::to_string(keep));
   if (best != 1 && best != 2) value_error("<group_best> must be 1 or 2, got " + std::to_string(best));
   if (bias) check_exactly(*bias, logits, {experts}, ScalarType::Float, "bias");
@@ -264,7 +263,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> plan(const Tensor& indices, int64_t e
   if (!indices.is_contiguous()) value_error("<indices> must be contiguous");
   const int64_t tokens = indices.size(0), k = indices.size(1), slots = tokens * k;
   check_experts(experts);
-  if (k < 1 || k > kMaxChoices) value_error("a token has 1 to 32 choices, got " + std::to_string(k));
+  if (k < 1 || k > DGN_MAX_CHOICES)
+    value_error("a token has 1 to " + std::to_string(DGN_MAX_CHOICES) + " choices, got " + std::to_string(k));
   if (align < 1 || align > INT32_MAX || slots > INT32_MAX || slots + std::min(experts, slots) * (align - 1) > INT32_MAX)
     value_error("<align> must be positive and the rows fewer than 2^31");
   Tensor counts = empty({experts}, ScalarType::Int, indices), offsets = empty({experts + 1}, ScalarType::Int, indices),
@@ -357,8 +357,8 @@ std::tuple<Tensor, Tensor> combine_grad(const Tensor& grad_output, const Tensor&
 }
 
 Tensor update_bias(const Tensor& bias, const Tensor& counts, double rate, const MaybeTensor& to) {
-  if (bias.dim() != 1 || bias.size(0) < 1 || bias.size(0) > kMaxExperts)
-    value_error("<bias> must be a vector of 1 to 1024 elements");
+  if (bias.dim() != 1 || bias.size(0) < 1 || bias.size(0) > DGN_MAX_EXPERTS)
+    value_error("<bias> must be a vector of 1 to " + std::to_string(DGN_MAX_EXPERTS) + " elements");
   check_cuda(bias, "bias");
   check_exactly(bias, bias, bias.sizes(), ScalarType::Float, "bias");
   check_exactly(counts, bias, bias.sizes(), ScalarType::Int, "counts");

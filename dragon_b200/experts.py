@@ -22,7 +22,7 @@ from dragon_b200 import _C
 from dragon_b200.comm import _enter_stream
 
 _SCORES = {"softmax": _C.SCORE_SOFTMAX, "sigmoid": _C.SCORE_SIGMOID}
-MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 32
+MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 32  # the DGN_MAX_ of include/dgn.h, for callers that size a model
 
 
 def _score_code(scores):

@@ -403,8 +403,12 @@ int dgn_rms_norm_grad(const void* grad_out, int64_t grad_out_stride, const void*
  * Choices are made as if computed in 64 bits, so that ranks and recomputations
  * agree.  An expert whose logit or key is -inf is not chosen; a NaN counts as
  * the largest key.  Slots that find no expert, and the tokens whose `mask` byte
- * is 0, get index -1 and weight 0.  1..1024 experts, k 1..32 and at most the
- * number of experts, 1..32 groups. */
+ * is 0, get index -1 and weight 0.  Limits of all calls of these operators: 1 to
+ * DGN_MAX_EXPERTS experts, k 1 to DGN_MAX_CHOICES and in the choice at most the
+ * number of experts, 1 to DGN_MAX_GROUPS groups. */
+#define DGN_MAX_EXPERTS 1024
+#define DGN_MAX_CHOICES 32
+#define DGN_MAX_GROUPS 32
 typedef enum { DGN_SCORE_SOFTMAX = 0, DGN_SCORE_SIGMOID = 1 } dgn_score;
 
 int dgn_route(const void* logits, int64_t stride, const float* bias, const uint8_t* mask, int32_t* indices,
