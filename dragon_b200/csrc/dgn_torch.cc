@@ -5,12 +5,15 @@
 //
 // Refusals are ValueError and TypeError as elsewhere in the package; a status of
 // the C-ABI becomes dragon_b200._C.DgnError.  Works on shapes, types and addresses
-// alone: nothing is copied, converted or synchronised, no autograd graph is recorded.
+// alone: nothing is copied, converted or synchronised, no autograd graph is recorded (of
+// which a caller whose inputs require gradients is told once).
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -111,6 +114,21 @@ int64_t matrix(const Tensor& t, const char* name, bool any_type = false) {
   return rows_of(t, name).stride;
 }
 
+const Tensor* maybe(const MaybeTensor& t) { return t ? &*t : nullptr; }
+// One warning of the process, for the mistake of taking a forward call for one that autograd follows.
+void tell_of_no_graph(const char* call, const char* backward, std::initializer_list<const Tensor*> inputs) {
+  static bool told = false;
+  if (told || !at::GradMode::is_enabled()) return;
+  for (const Tensor* t : inputs) {
+    if (!t || !t->requires_grad()) continue;
+    const std::string what = std::string(call) + ": an input requires a gradient, but the call records no autograd graph; its backward pass is " +
+                             backward + " (call both in a torch.autograd.Function, or the forward call under torch.no_grad())";
+    if (PyErr_WarnEx(PyExc_UserWarning, what.c_str(), 1) != 0) throw py::error_already_set();
+    told = true;
+    return;
+  }
+}
+
 // ---- norm ------------------------------------------------------------------------------
 
 void check_norm_input(const Tensor& x, const char* name) {
@@ -136,6 +154,7 @@ std::tuple<Tensor, Tensor, Tensor, MaybeTensor> rms_norm(const Tensor& x, const 
                                                           std::optional<ScalarType> out_type, int64_t group,
                                                           bool in_place) {
   check_norm_input(x, "x");
+  tell_of_no_graph("rms_norm", "rms_norm_grad", {&x, maybe(weight), maybe(residual)});
   const Rows r = rows_of(x, "x");
   if (!(eps >= 0x1p-126) || eps > 3.4e38) value_error("<eps> must be a positive number, 2^-126 at least");
   if (group != 0 && group != 32 && group != 64 && group != 128)
@@ -228,6 +247,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const MaybeTen
                                  int score, int64_t groups, int64_t keep, int64_t best, bool renormalize, double scale) {
   const int64_t stride = matrix(logits, "logits"), tokens = logits.size(0), experts = logits.size(1);
   check_choice(k, experts);
+  tell_of_no_graph("route", "route_grad", {&logits});
   if (groups < 1 || groups > DGN_MAX_GROUPS || experts % groups)
     value_error("<groups> must be 1 to " + std::to_string(DGN_MAX_GROUPS) + " and divide the number of experts");
   if (keep < 1 || keep > groups) value_error("<keep_groups> must be 1 to <groups>, got " + std::to_string(keep));
@@ -295,6 +315,7 @@ Tensor dispatch(const Tensor& x, const Tensor& offsets, const Tensor& ends, cons
   const Plan p = {offsets, ends, positions};
   const int64_t stride = matrix(x, "x", true), tokens = x.size(0), cols = x.size(1), size = x.element_size();
   check_plan(p, x);
+  tell_of_no_graph("dispatch", "dispatch_grad", {&x});
   if (tokens != p.tokens())
     value_error("<x> must have the plan's " + std::to_string(p.tokens()) + " rows, got " + std::to_string(tokens));
   if (cols == 0) value_error("<x> has no columns");
@@ -330,6 +351,7 @@ Tensor combine(const Tensor& rows, const Tensor& offsets, const Tensor& ends, co
                const MaybeTensor& weights, const MaybeTensor& residual) {
   const Plan p = {offsets, ends, positions};
   const int64_t cols = check_rows(rows, p);
+  tell_of_no_graph("combine", "combine_grad", {&rows, maybe(weights), maybe(residual)});
   if (weights) check_exactly(*weights, rows, {p.tokens(), p.k()}, ScalarType::Float, "weights");
   const int64_t residual_stride = residual ? of_tokens(*residual, rows, p, "residual") : 0;
   Tensor out = empty({p.tokens(), cols}, rows.scalar_type(), rows);

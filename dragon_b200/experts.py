@@ -15,7 +15,9 @@ dgn_expert_* of include/dgn.h).
 
 Like the collectives these calls enqueue work on a stream and return: nothing
 is synchronised, so the number of rows of each expert stays on the device, and
-no autograd graph is recorded, the backward pass is the ``_grad`` calls.
+no autograd graph is recorded, the backward pass is the ``_grad`` calls (a
+process that passes tensors which require gradients, with gradients enabled, is
+warned once).
 """
 
 from dragon_b200 import _C

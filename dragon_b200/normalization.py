@@ -8,7 +8,8 @@ activations moves them at half the bytes of bfloat16
 (``comm.all_gather(r.output.view(torch.uint8), ...)``).
 
 Like the collectives these calls enqueue work on a stream and return; no
-autograd graph is recorded, the backward pass is the ``_grad`` call.
+autograd graph is recorded, the backward pass is the ``_grad`` call (a process
+that passes tensors which require gradients, with gradients enabled, is warned once).
 """
 
 import collections

@@ -1,5 +1,9 @@
 """Calls at the edges of what the norm and expert operators take."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -50,3 +54,40 @@ def test_the_longest_odd_rows(dgn_lib):
     residual[:, :64] = 3.0
     cut = residual[:, 1:cols + 2]
     assert torch.equal(combine(row, one, residual=cut), cut + 1)
+
+
+def test_a_process_is_told_once_that_no_graph_is_recorded(dgn_lib):
+    code = """
+import warnings
+import torch
+from dragon_b200.experts import combine, dispatch, plan, route
+from dragon_b200.normalization import rms_norm, rms_norm_grad
+x = torch.ones(4, 8, device="cuda:0", requires_grad=True)
+p = plan(torch.zeros(4, 1, dtype=torch.int32, device="cuda:0"), 2)
+calls = [lambda x: rms_norm(x).output, lambda x: rms_norm(x.detach(), x[0]).output, lambda x: route(x, 2)[1], lambda x: dispatch(x, p),
+         lambda x: combine(x, p)]
+def run(inputs):
+    with warnings.catch_warnings(record=True) as told:
+        warnings.simplefilter("always")
+        for call in calls:
+            assert not call(inputs).requires_grad
+    return [str(w.message) for w in told]
+assert run(x.detach()) == []
+with torch.no_grad():
+    assert run(x) == []
+for call in calls:  # a filter that makes it an error stops every one of them
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        try:
+            call(x)
+        except UserWarning:
+            continue
+        raise AssertionError("no word")
+told = run(x)
+assert len(told) == 1 and "rms_norm_grad" in told[0], told
+assert run(x) == []
+print("TOLD_ONCE")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "TOLD_ONCE" in done.stdout, done.stdout + done.stderr
