@@ -7,7 +7,7 @@ import sys
 import pytest
 import torch
 
-from dragon_b200.experts import combine, dispatch, plan, route
+from dragon_b200.experts import combine, combine_grad, dispatch, plan, route
 from dragon_b200.normalization import rms_norm, rms_norm_grad
 
 pytestmark = pytest.mark.gpu
@@ -60,7 +60,7 @@ def test_a_process_is_told_once_that_no_graph_is_recorded(dgn_lib):
     code = """
 import warnings
 import torch
-from dragon_b200.experts import combine, dispatch, plan, route
+from dragon_b200.experts import combine, combine_grad, dispatch, plan, route
 from dragon_b200.normalization import rms_norm, rms_norm_grad
 x = torch.ones(4, 8, device="cuda:0", requires_grad=True)
 p = plan(torch.zeros(4, 1, dtype=torch.int32, device="cuda:0"), 2)
@@ -91,3 +91,30 @@ print("TOLD_ONCE")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert "TOLD_ONCE" in done.stdout, done.stdout + done.stderr
+
+
+U = 2.0 ** -24  # half a step of float32
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [64, 61])
+@pytest.mark.parametrize("start", [0, 1, 8])
+def test_strided_rows_against_the_definition(dgn_lib, dtype, cols, start):
+    """Whatever the order: a sum of n products is within n steps' halves of the sum of their magnitudes, then rounded once."""
+    g = torch.Generator().manual_seed(1)
+    indices = torch.stack([torch.randperm(6, generator=g)[:3] for _ in range(40)]).int().to(DEV)
+    p = plan(indices, 6)
+    rows, weights, wide = normal(120, cols, seed=2, dtype=dtype), normal(40, 3, seed=3), normal(40, 90, seed=4, dtype=dtype)
+    cut, mine = wide[:, start:start + cols], rows[p.positions.long()].double()
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * half  # below the normal numbers steps stop shrinking
+    terms = mine * weights.double()[:, :, None]
+    want, size = terms.sum(1) + cut.double(), terms.abs().sum(1) + cut.double().abs()
+    got = combine(rows, p, weights, cut).double()
+    assert ((got - want).abs() <= 4 * U * size + half * (want.abs() + 4 * U * size) + tiny).all()
+    grad_rows, grad_weights = combine_grad(cut, rows, p, weights)
+    terms = mine * cut.double()[:, None]
+    assert ((grad_weights.double() - terms.sum(2)).abs() <= cols * U * terms.abs().sum(2)).all()
+    want = weights.double()[:, :, None] * cut.double()[:, None]
+    off = (grad_rows[p.positions.long()].double() - want).abs()
+    assert (off <= U * want.abs() + half * (1 + U) * want.abs() + tiny).all()
