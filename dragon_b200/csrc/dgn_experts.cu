@@ -6,8 +6,8 @@
 // No matrix product is involved.  The moves are bound by memory: 65536 slots of 2048
 // bfloat16 columns take 50 us to dispatch (93 % of the measured copy rate), 55 to combine with a
 // residual (94 %), 98 for the backward pass (90 %), 48 without weights (98 %).  The choice is
-// bound by its instructions: 65536 tokens of 128 float32 logits take 22 us, the bytes 5.8; its
-// gradient 15.7 of 11.0.
+// bound by the latency of its dependent maxima: 65536 tokens of 128 float32 logits take 21 us,
+// the bytes 5.8; its gradient 18 of 11.0, for the instructions of expf.
 #include <math.h>
 
 #include "dgn_kernels.cuh"
@@ -79,7 +79,9 @@ __device__ __noinline__ void exact_scores(double* v, int sigmoid, double top, do
 
 // One token's choice in 64 bits by a whole warp, its keys' orders in shared memory.  Taken by the
 // tokens whose choice hangs on values that float32 does not tell apart, and by those that
-// hold a NaN or an infinity: about one in a thousand, but a small batch waits for that one.
+// hold a NaN or an infinity: about one in a thousand of random logits, but a small batch waits for
+// that one.  Float32 rows with more equal logits at the border than it can put in order go here
+// too, though their order is plain: 65536 tokens of 128 equal logits take 188 us, 21 of random ones.
 template <typename T>
 __device__ __noinline__ void route_exact(const RouteParams& p, long long token, u64* key) {
   const int lane = threadIdx.x & 31, experts = p.experts;
@@ -330,11 +332,14 @@ __host__ __device__ inline int route_shared(int experts, int groups, int teams) 
 
 // L lanes for a token, N experts for a lane; experts <= 1 << bits <= L * N.
 //
-// What bounds it is the number of instructions (k passes over each logit), not the bytes: 65536
-// tokens of 128 float32 logits take 22 us, of 256 with a bias 50, four to five times their bytes; blocks are held to
-// 64 registers so that eight share an SM.  A key in float32 and its expert's number are one 31-bit word: the key's order without its lowest bits, which hold the number, the lowest
-// the largest.  So the words differ, one maximum finds value and place at once, and the
-// next largest is the largest of word - last, wrapped around, without anything being marked.
+// What bounds it is latency, not the bytes: k + 1 rounds, each a maximum over a lane's words and a chain of
+// shuffles that waits for it (0.6 of the issue slots at 43 % of the warps).  65536 tokens of 128 float32
+// logits take 21 us, of 256 with a bias 58, four to six times their bytes; blocks are held to 64 registers
+// so that eight share an SM.
+//
+// A key in float32 and its expert's number are one 31-bit word: the key's order without its lowest bits,
+// which hold the number, the lowest the largest.  So the words differ, one maximum finds value and place at
+// once, and the next largest is the largest of word - last, wrapped around, without anything being marked.
 // With a bias the upper bits are not the key's order but its distance from the row's largest
 // in even steps, as fine as the scores are exact.  The choice stands if each of the k + 1
 // first words is clear of the next: by what its upper bits leave open, and by the rounding of the
@@ -610,7 +615,7 @@ struct RouteGradParams {
 // The gradient of the scores is zero but for the k choices: those are put into a row of
 // shared memory, and each lane picks up its own experts'.  The softmax's exponentials are expf's for float32: those of
 // the unit alone are off by more the smaller the score is (4e-6 of one 80 below the row's largest), far less than the
-// rounding of a 16-bit gradient.  65536 tokens of 128 logits: 16.4 us in float32 (13.3 by the unit), 14.0 in bfloat16.
+// rounding of a 16-bit gradient.  65536 tokens of 128 logits: 17.9 us in float32 (15.1 by the unit), 14.6 in bfloat16.
 template <typename T, int L, int N, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads) route_grad_kernel(const __grid_constant__ RouteGradParams p) {
   constexpr int Q = kMaxChoices / L, V = VEC ? 16 / (int)sizeof(T) : 1;

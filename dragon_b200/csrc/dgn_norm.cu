@@ -13,12 +13,12 @@
 // Sums are held in 32 bits.  A row is read once: it stays in registers, packed in
 // its storage type, between the sum of squares and the output.
 //
-// Bound by memory: 8192 rows of 4096 bfloat16 columns with a residual take 42.8 us forward
+// Bound by memory: 8192 rows of 4096 bfloat16 columns with a residual take 42.9 us forward
 // (6.3 TB/s, 97 % of the measured copy rate) and 44.8 us backward (93 %: 41 without the
-// weight gradient, whose partial sums go through the second cache and a second kernel).  With 8-bit output it
-// is the instructions, 42.7 us for bytes of 36.3: each value is rounded, multiplied, compared and
-// converted.  Rows that are not aligned move by single or paired elements and
-// are bound by their number: 4097 columns take 95 us forward, 278 backward.
+// weight gradient, whose partial sums go through the second cache and a second kernel).
+// With 8-bit output it is the instructions, 44.7 us for bytes of 36.3: each value is rounded,
+// multiplied twice, compared and converted.  Rows that are not aligned move by single or
+// paired elements and are bound by their number: 4097 columns take 96 us forward, 277 backward.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -673,7 +673,8 @@ struct RowShape {
   int lanes() const { return teams > 1 ? team : 0; }  // the kernels' TEAM
 };
 
-// Two parts a thread up to 512: with four, 4096 columns of bfloat16 in 8 bits took 45.0 us instead of 42.6.
+// Two parts a thread up to 512: with four, 4096 columns of bfloat16 in 8 bits took 45.0 us instead of 42.6 (codes of one
+// rounded factor; 44.7 with the quotient and its remainder's).
 // Rows of up to 128 parts go to a warp or a half or quarter of one and need no barrier; longer ones to a block, with
 // more parts for a thread where the threads would pass 512.
 RowShape row_shape(int cols, int elems, bool vec) {

@@ -72,8 +72,9 @@ class ExpertPlan(object):
     counts [experts], the rows of each expert (the caller's to change: an
     all-reduce may add up the group's in place); offsets [experts + 1], the first
     row of each expert's block, a multiple of `align`, and the end of the last;
-    ends [experts], behind the last row in use of each block; positions [tokens, k], the row of each choice, -1 for none.  `capacity` is the
-    number of rows that always suffices."""
+    ends [experts], behind the last row in use of each block; positions [tokens, k],
+    the row of each choice, -1 for none.  `capacity` is the number of rows that
+    always suffices."""
 
     def __init__(self, counts, offsets, ends, positions, align):
         self.counts, self.offsets, self.ends, self.positions, self.align = counts, offsets, ends, positions, align
@@ -100,7 +101,8 @@ def dispatch(x, plan, out=None, stream=None):
     x: [tokens, columns] of any type (8-bit codes and their scales are two calls
     with one plan).  out: [rows, columns], by default new with plan.capacity rows; a
     shorter one takes the rows that it has.  The unused rows of an expert's block
-    become zeros, rows behind the last block stay as they are."""
+    become zeros, rows behind the last block stay as they are: in a new tensor
+    whatever its memory held."""
     if stream is not None:
         with _enter_stream(stream, x.device):
             return dispatch(x, plan, out)

@@ -367,14 +367,15 @@ int dgn_allreduce_static_status(int clear);
  * dgn_rms_norm: hidden = x + residual (rounded to `dtype`; without a residual
  * hidden is x itself and not written), rstd = 1/sqrt(mean(hidden^2) + eps),
  * out = hidden * rstd * weight.  dtype: DGN_F16, DGN_BF16, DGN_F32; 1..32768
- * columns; eps 2^-126 at least.  The weight may be NULL; its type is float32 or `dtype`.  hidden may
- * be the residual's own memory, with the same stride.  The sum of a row's squares
- * is held in float32: rows where it passes 3.4e38 (4096 columns of 2.9e17 each)
- * come out as zeros, with rstd 0.  With a code, out holds 8-bit values instead and
- * scales one float32 per row and group of `group` columns (32, 64, 128, or 0: the row):
- * value = code * scale, scale = largest magnitude / largest code (127, 448,
- * 57344), groups below 2^-40 taking that bound's scale; a group with a NaN or an
- * infinity has scale NaN.  out, scales [rows, groups] and rstd are contiguous. */
+ * columns; eps 2^-126 at least.  The weight may be NULL; its type is float32 or
+ * `dtype`.  hidden may be the residual's own memory, with the same stride.  The sum
+ * of a row's squares is held in float32: rows where it passes 3.4e38 (4096 columns
+ * of 2.9e17 each) come out as zeros, with rstd 0.  With a code, out holds 8-bit
+ * values instead and scales one float32 per row and group of `group` columns (32,
+ * 64, 128, or 0: the row): value = code * scale, scale = largest magnitude /
+ * largest code (127, 448, 57344), groups below 2^-40 taking that bound's scale; a
+ * group with a NaN or an infinity has scale NaN.  out, scales [rows, groups] and
+ * rstd are contiguous. */
 typedef enum { DGN_CODE_NONE = 0, DGN_CODE_I8 = 1, DGN_CODE_E4M3 = 2, DGN_CODE_E5M2 = 3 } dgn_code;
 
 int dgn_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
@@ -426,9 +427,10 @@ int dgn_route_grad(const float* grad_weights, const void* logits, int64_t stride
  * goes when rows are put in the order of their experts, equal ones in the order
  * of the slots.  Expert e's rows start at offsets[e], a multiple of `align`;
  * counts[e] of them are in use, the last before ends[e] = offsets[e] + counts[e];
- * offsets[e+1] begins the next block and offsets[experts] ends the last.  positions[slot] is -1 for an index outside
- * 0..experts-1.  slots + min(experts, slots) * (align - 1) rows suffice (below
- * 2^31).  `workspace`: dgn_expert_plan_workspace bytes (may be 0). */
+ * offsets[e+1] begins the next block and offsets[experts] ends the last.
+ * positions[slot] is -1 for an index outside 0..experts-1.
+ * slots + min(experts, slots) * (align - 1) rows suffice (below 2^31).
+ * `workspace`: dgn_expert_plan_workspace bytes (may be 0). */
 int64_t dgn_expert_plan_workspace(int64_t slots, int experts);
 int dgn_expert_plan(const int32_t* indices, int64_t slots, int experts, int align, int32_t* counts, int32_t* offsets,
                     int32_t* ends, int32_t* positions, void* workspace, int64_t workspace_bytes, int device, void* stream);
