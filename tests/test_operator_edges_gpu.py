@@ -118,3 +118,29 @@ def test_strided_rows_against_the_definition(dgn_lib, dtype, cols, start):
     want = weights.double()[:, :, None] * cut.double()[:, None]
     off = (grad_rows[p.positions.long()].double() - want).abs()
     assert (off <= U * want.abs() + half * (1 + U) * want.abs() + tiny).all()
+
+
+def test_offsets_beyond_32_bits(dgn_lib):
+    """Matrices of more than 2^32 bytes and 2^31 elements: their last rows are those of a small call with the same layout."""
+    rows, cols, last = 530000, 4104, 300
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[:], x[-last:] = 1.0, normal(last, cols, seed=1, dtype=torch.bfloat16)
+    weight = 1 + 0.1 * normal(cols, seed=2)
+    for dtype, group in ((None, 0), (torch.float8_e4m3fn, 32)):
+        big, small = (rms_norm(t, weight, out_dtype=dtype, group_size=group) for t in (x, x[-last:]))
+        assert torch.equal(big.output[-last:].view(torch.uint8), small.output.view(torch.uint8))
+        assert torch.equal(big.rstd[-last:], small.rstd) and (dtype is None or torch.equal(big.scale[-last:], small.scale))
+    assert torch.equal(rms_norm_grad(x, x, big.rstd)[0][-last:], rms_norm_grad(x[-last:], x[-last:], small.rstd)[0])
+    del big
+    indices = torch.zeros(rows, 1, dtype=torch.int32, device=DEV)
+    indices[-last:] = 1  # the second expert's block begins behind 2^31 elements
+    p = plan(indices, 2)
+    moved = dispatch(x, p)
+    assert torch.equal(p.positions[-last:, 0], torch.arange(rows - last, rows, dtype=torch.int32, device=DEV))
+    assert torch.equal(moved[-last:], x[-last:])
+    weights = torch.full((rows, 1), 0.5, device=DEV)
+    assert torch.equal(combine(moved, p, weights)[-last:], x[-last:] * 0.5)
+    grad_rows, grad_weights = combine_grad(x, moved, p, weights)
+    assert torch.equal(grad_rows[-last:], x[-last:] * 0.5)
+    want = x[-last:].double().square().sum(1)
+    assert ((grad_weights[-last:, 0].double() - want).abs() <= cols * U * want).all()
